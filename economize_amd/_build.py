@@ -22,7 +22,8 @@ CSRC = HERE / "csrc"
 LIBRARY = HERE / "libeconomize_amd.so"
 SOURCES = ["capi.hip", "paged_attention.hip", "paged_attention_f16.hip", "kv_quant.hip", "quest.hip", "kivi.hip",
            "kivi_quantize.hip", "dense_attention.hip", "gather.hip", "kivi_dense.hip", "kivi_cells.hip",
-           "kivi_verify.hip", "kivi_packed.hip"]
+           "kivi_verify.hip", "kivi_packed.hip", "capi_prompt.hip", "prompt_attention.hip", "attention_mass.hip",
+           "eviction.hip", "heavy_hitter.hip"]
 
 FLAGS = [
     "--offload-arch=gfx950",

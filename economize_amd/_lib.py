@@ -7,6 +7,7 @@ The library is loaded on first use and never replaced by anything else: if it is
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
@@ -95,9 +96,20 @@ SIGNATURES: dict[str, tuple[type | None, list]] = {
                                          _P, _P, _I, _I, _I,  # counts, bits, groups
                                          _P, _L, _L, _L, _L, _P, _P, _L, _L, _L,  # mask, sinks, out
                                          _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _S, _P]),
+    "eco_prompt_attention_workspace_size": (c_size_t, [_I, _I, _I, _I, _I, _I]),
+    "eco_prompt_attention": (c_int32, [_P, _I, _L, _L, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _I, _I,
+                                       _P, _P, _L, _L, _P, _L, _I, _I, _I, _I, _F, _F, _P, _S, _P]),
+    "eco_attention_mass": (c_int32, [_P, _I, _L, _L, _P, _L, _L, _P, _L, _P, _P, _P, _P, _I, _L, _L, _I, _I, _I,
+                                     _P, _L, _I, _I, _I, _I, _F, _F, _P]),
+    "eco_evict_prompt": (c_int32, [_P, _P, _L, _L, _L, _L, _P, _L, _P, _P, _L, _I, _P, _P, _P, _P, _P, _P,
+                                   _I, _I, _I, _I, _I, _I, _P]),
+    "eco_heavy_hitter_workspace_size": (c_size_t, [_I, _I, _I, _I, _I]),
+    "eco_heavy_hitter_decode": (c_int32, [_P, _I, _L, _L, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P,
+                                          _P, _L, _L, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _S, _P]),
 }
 
 _lib: ctypes.CDLL | None = None
+_HERE = contextlib.nullcontext()
 
 
 def lib() -> ctypes.CDLL:
@@ -142,6 +154,13 @@ def stream_of(device: torch.device) -> int:
     0.1 us where ``torch.cuda.current_stream`` builds a stream object in 2.0."""
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def on(device: torch.device) -> contextlib.AbstractContextManager:
+    """``device`` as the current one for a launch (nothing to do when it is already)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

@@ -1,0 +1,132 @@
+// Device pieces shared by the packed-prompt kernels: 32x32x16 products, K/V tiles in LDS, the rows of a sequence.
+#pragma once
+
+#include "prompt.hpp"
+
+namespace eco {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int FMT>
+__device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+    if constexpr (FMT == BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+}
+
+// Two floats as a pair of bf16 or fp16, rounded to nearest even.
+template <int FMT>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    if constexpr (FMT == BF16) {
+        bf16x2 r;
+        r[0] = static_cast<__bf16>(a);
+        r[1] = static_cast<__bf16>(b);
+        return __builtin_bit_cast(uint32_t, r);
+    } else {
+        f16x2 r;
+        r[0] = static_cast<_Float16>(a);
+        r[1] = static_cast<_Float16>(b);
+        return __builtin_bit_cast(uint32_t, r);
+    }
+}
+
+__device__ __forceinline__ float swap_max(float x) {  // the larger of lanes l and l ^ 32
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_nan(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float swap_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The bounds of one sequence, clamped to the rows of the tensors.
+struct Sequence {
+    int64_t q0, k0;
+    int nq, nk;
+};
+
+__device__ __forceinline__ Sequence sequence_of(const PackedRows& r, int s) {
+    auto clamp = [](int64_t x, int64_t hi) { return x < 0 ? 0 : (x > hi ? hi : x); };
+    Sequence q;
+    q.q0 = clamp(r.q_begin[s], r.q_rows);
+    q.nq = static_cast<int>(clamp(r.q_end[s], r.q_rows) - q.q0);
+    q.k0 = clamp(r.k_begin[s], r.k_rows);
+    q.nk = static_cast<int>(clamp(r.k_end[s], r.k_rows) - q.k0);
+    if (q.nq < 0) q.nq = 0;
+    if (q.nk < 0) q.nk = 0;
+    return q;
+}
+
+// A tile of 64 rows of D 16-bit channels in LDS, in chunks of 16 bytes. Keys are read as MFMA operands of 32 rows by 16
+// channels (ds_read_b128, lane l row l % 32), values transposed (ds_read_b64_tr_b16, 4 rows by 64 bytes for 32 lanes); the
+// two swizzles spread the rows of one such read over all 64 banks.
+template <int D>
+struct Tile {
+    static constexpr int CHUNKS = D / 8;
+    static constexpr int BYTES = 64 * D * 2;
+    static __device__ __forceinline__ int key_chunk(int row, int chunk) {
+        return CHUNKS == 8 ? chunk ^ ((row >> 1) & 7) : chunk ^ (row & 15);
+    }
+    static __device__ __forceinline__ int value_chunk(int row, int chunk) {
+        return CHUNKS == 8 ? chunk ^ (((row >> 1) & 1) << 2) : chunk ^ ((row & 3) << 2);
+    }
+};
+
+// Rows [row0, row0 + 64) of a sequence's keys or values into registers: rows past its end read as zero (the buffer
+// resource ends with the sequence).
+template <int D, int THREADS>
+struct TileLoad {
+    static constexpr int N = 64 * (D / 8) / THREADS;
+    uint4 x[N];
+
+    __device__ __forceinline__ void load(const uint16_t* base, int64_t stride, int row0, int rows, int tid) {
+        const int left = rows - row0;
+        const int n = left < 64 ? left : 64;
+        const uint32_t bytes = n <= 0 ? 0u : static_cast<uint32_t>((n - 1) * stride * 2 + D * 2);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(base + static_cast<int64_t>(row0) * stride), 0, bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + i * THREADS;
+            const uint32_t off = static_cast<uint32_t>(c / (D / 8)) * static_cast<uint32_t>(stride * 2) +
+                                 static_cast<uint32_t>(c % (D / 8)) * 16u;
+            x[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
+        }
+    }
+
+    // Infinities and NaN to 0; whether there was one.
+    template <int FMT>
+    __device__ __forceinline__ bool drop_non_finite() {
+        constexpr uint32_t LIMIT = FMT == BF16 ? 0x7F80u : 0x7C00u;
+        uint32_t big = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t m = max_magnitude8(x[i]);
+            big = m > big ? m : big;
+        }
+        if (big < LIMIT) return false;
+        auto clean = [](uint32_t w) {
+            return ((w & 0x7FFFu) >= LIMIT ? 0u : w & 0xFFFFu) | ((w >> 16 & 0x7FFFu) >= LIMIT ? 0u : w & 0xFFFF0000u);
+        };
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = make_uint4(clean(x[i].x), clean(x[i].y), clean(x[i].z), clean(x[i].w));
+        return true;
+    }
+
+    template <bool KEYS>
+    __device__ __forceinline__ void store(uint8_t* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + i * THREADS;
+            const int row = c / (D / 8), chunk = c % (D / 8);
+            const int to = KEYS ? Tile<D>::key_chunk(row, chunk) : Tile<D>::value_chunk(row, chunk);
+            *reinterpret_cast<uint4*>(lds + row * (D * 2) + to * 16) = x[i];
+        }
+    }
+};
+
+}  // namespace eco

@@ -1,0 +1,189 @@
+"""Attention over whole prompts on the GPU: packed sequences of different lengths, and the weight every key received.
+
+The reference's kernels take up to 64 queries (attention/interface.py:243-285) and leave prompts to ``sdpa``, which
+takes one padded batch; these take packed rows and give the softmax statistics an eviction by accumulated attention
+weight needs (:mod:`economize_amd.eviction`).
+
+Sequences are given by ``cu_seqlens``, int32 ``[N + 1]`` on the device (sequence ``s`` holds rows ``cu[s] .. cu[s + 1]``), or
+by a pair ``(begin, end)`` of int32 ``[N]`` (sequences in order and apart, rows between them belonging to none: a padded
+batch). ``max_seqlen`` is the longest one (it sizes the launch; the number of rows when it is not known).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Union
+
+import torch
+
+from . import _lib
+from .decode import sinks_operand
+from .errors import ConfigError
+
+__all__ = ["Rows", "attention_mass", "prompt_attention"]
+
+#: Rows of the sequences: ``cu_seqlens`` or ``(begin, end)``.
+Rows = Union[torch.Tensor, tuple[torch.Tensor, torch.Tensor]]
+
+DTYPES = (torch.bfloat16, torch.float16)
+
+
+def row_bounds(rows: Rows, device: torch.device) -> tuple[torch.Tensor, int, int, int]:
+    """A tensor that keeps the bounds alive, the addresses of every sequence's first and past-the-end row, and how many
+    sequences there are."""
+    if torch.is_tensor(rows):
+        if rows.dtype != torch.int32 or rows.dim() != 1 or rows.numel() < 2 or rows.stride(0) != 1:
+            raise ConfigError("cu_seqlens must be contiguous int32 [sequences + 1] with at least one sequence")
+        if rows.device != device:
+            raise ConfigError(f"cu_seqlens on {rows.device}, the queries on {device}")
+        at = rows.data_ptr()
+        return rows, at, at + 4, rows.numel() - 1
+    begin, end = rows
+    for t in (begin, end):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 1 or t.stride(0) != 1 or t.device != device:
+            raise ConfigError(f"begin and end must be contiguous int32 [sequences] on {device}")
+    if begin.numel() != end.numel():
+        raise ConfigError(f"{begin.numel()} sequences begin, {end.numel()} end")
+    return begin, begin.data_ptr(), end.data_ptr(), begin.numel()
+
+
+def operand(x: torch.Tensor) -> torch.Tensor:
+    """``x`` ``[..., D]`` as the kernels read it: unit channel stride, base and other strides whole 16 bytes from 0 to below
+    2^24 elements (a copy only when it is not)."""
+    es = x.element_size()
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
+            n == 1 or (0 <= s < 1 << 24 and (s * es) % 16 == 0) for n, s in zip(x.shape[:-1], x.stride()[:-1])):
+        return x
+    return x.contiguous()
+
+
+def strides_of(x: torch.Tensor) -> tuple[int, int]:
+    """The first two strides; that of an axis of one entry is not used and may be anything, so it is given as 0."""
+    return tuple(0 if n == 1 else s for n, s in zip(x.shape[:2], x.stride()[:2]))
+
+
+def _check(what: str, query: torch.Tensor, key: torch.Tensor) -> None:
+    if query.dim() != 3 or key.dim() != 3 or query.shape[2] != key.shape[2]:
+        raise ConfigError(f"{what} takes queries [T, Hq, D] and keys [Tk, Hkv, D], got {tuple(query.shape)} and "
+                          f"{tuple(key.shape)}")
+    if query.dtype not in DTYPES or key.dtype != query.dtype:
+        raise ConfigError(f"{what} takes bf16 or fp16 queries and keys of one dtype, got {query.dtype} and {key.dtype}")
+    if key.shape[1] == 0 or query.shape[1] % key.shape[1] or query.shape[1] == 0:
+        raise ConfigError(f"{query.shape[1]} query heads are not a multiple of {key.shape[1]} KV heads")
+
+
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: Rows,
+                     max_seqlen: int | None = None, scale: float | None = None, *, cu_seqlens_k: Rows | None = None,
+                     max_seqlen_k: int | None = None, softcap: float | None = None, sinks: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None, return_lse: bool = False
+                     ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Causal attention of packed sequences: query ``i`` of a sequence of ``nq`` queries and ``nk`` keys sees its keys
+    ``j <= i + nk - nq`` (the queries are its last tokens, so a prompt may be given in chunks behind its earlier keys).
+
+    Args:
+        query: ``[T, Hq, D]`` (any strides), bf16 or fp16, head dim 64, 128 or 256.
+        key, value: ``[Tk, Hkv, D]`` in the query's dtype.
+        cu_seqlens: The sequences' query rows (see the module).
+        max_seqlen: The longest sequence's queries.
+        scale: Multiplier of the scores, positive (``1 / sqrt(D)``).
+        cu_seqlens_k: The sequences' key rows, when they are not the query rows.
+        max_seqlen_k: The longest sequence's keys.
+        softcap: Optional tanh soft cap of the scaled scores.
+        sinks: Optional ``[Hq]`` attention-sink logits.
+        out: Optional ``[T, Hq, D]`` output buffer; rows of no sequence are left as they are.
+        return_lse: Also return the logarithm of every softmax denominator, fp32 ``[Hq, T]``.
+
+    Returns:
+        ``[T, Hq, D]`` in the query's dtype (and the denominators' logarithms). A query that sees no key, and without
+        ``out`` a row of no sequence, gives 0 and ``-inf``. Nothing here is differentiated.
+    """
+    device = _lib.require_gpu(query, key, value)
+    _check("prompt_attention", query, key)
+    if value.shape != key.shape or value.dtype != key.dtype:
+        raise ConfigError(f"values {tuple(value.shape)} {value.dtype} do not match the keys {tuple(key.shape)} {key.dtype}")
+    tokens, q_heads, head_dim = query.shape
+    keep_q, q_begin, q_end, sequences = row_bounds(cu_seqlens, device)
+    keep_k, k_begin, k_end, k_sequences = (keep_q, q_begin, q_end, sequences) if cu_seqlens_k is None else \
+        row_bounds(cu_seqlens_k, device)
+    if k_sequences != sequences:
+        raise ConfigError(f"{sequences} sequences of queries, {k_sequences} of keys")
+    if cu_seqlens_k is None and key.shape[0] != tokens:
+        raise ConfigError(f"{key.shape[0]} keys for {tokens} queries need cu_seqlens_k")
+    sinks = sinks_operand(sinks, q_heads)
+    if sinks is not None and sinks.device != device:
+        raise ConfigError(f"sinks on {sinks.device}, the queries on {device}")
+    fill = out is None
+    if out is None:
+        out = torch.empty(tokens, q_heads, head_dim, dtype=query.dtype, device=device)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or operand(out) is not out:
+        raise ConfigError("out must be [T, Hq, D] in the query's dtype on its device, channels contiguous and rows on 16 "
+                          "bytes")
+    lse = torch.empty(q_heads, tokens, dtype=torch.float32, device=device) if return_lse else None
+    if return_lse and not fill:
+        lse.fill_(-math.inf)
+    query, key, value = operand(query), operand(key), operand(value)
+    max_q = tokens if max_seqlen is None else min(int(max_seqlen), tokens)
+    max_k = key.shape[0] if max_seqlen_k is None else min(int(max_seqlen_k), key.shape[0])
+    if cu_seqlens_k is None and max_seqlen_k is None:
+        max_k = max_q
+    with _lib.on(device):
+        need = int(_lib.lib().eco_prompt_attention_workspace_size(sequences, max_q, max_k, q_heads, key.shape[1], head_dim))
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _lib.call(
+            "eco_prompt_attention", query.data_ptr(), _lib.fmt(query.dtype), *strides_of(query), key.data_ptr(),
+            value.data_ptr(), *strides_of(key), *strides_of(value), q_begin, q_end, k_begin, k_end, sequences, tokens,
+            key.shape[0], max_q, max_k, _lib.ptr(sinks), out.data_ptr(), *strides_of(out), _lib.ptr(lse), tokens,
+            int(fill), q_heads, key.shape[1], head_dim, float(1 / math.sqrt(head_dim) if scale is None else scale),
+            float(softcap or 0.0), _lib.ptr(ws), need, _lib.stream_of(device))
+    return (out, lse) if return_lse else out
+
+
+def attention_mass(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu_seqlens: Rows,
+                   max_seqlen: int | None = None, scale: float | None = None, *, cu_seqlens_k: Rows | None = None,
+                   max_seqlen_k: int | None = None, window: int | None = None, softcap: float | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """The attention weight every key of packed sequences received, fp32 ``[Hkv, Tk]``: the sum over the queries that see
+    the key and the query heads of its KV head of ``exp(score - lse)``, in a fixed order.
+
+    Args:
+        query, key, cu_seqlens, max_seqlen, scale, cu_seqlens_k, max_seqlen_k, softcap: As :func:`prompt_attention` took
+            them.
+        lse: fp32 ``[Hq, T]``, as :func:`prompt_attention` returned it.
+        window: Count only the last ``window`` queries of every sequence (an observation window).
+        out: Optional fp32 ``[Hkv, Tk]`` output buffer; keys of no sequence are left as they are (without it they give 0).
+    """
+    device = _lib.require_gpu(query, key, lse)
+    _check("attention_mass", query, key)
+    tokens, q_heads, head_dim = query.shape
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (q_heads, tokens) or (tokens > 1 and lse.stride(1) != 1) or \
+            (q_heads > 1 and lse.stride(0) < tokens):
+        raise ConfigError(f"lse must be fp32 [{q_heads}, {tokens}] with contiguous rows apart")
+    if window is not None and (isinstance(window, bool) or int(window) != window or window < 1):
+        raise ConfigError(f"window must be a positive integer or None, got {window!r}")
+    keep_q, q_begin, q_end, sequences = row_bounds(cu_seqlens, device)
+    keep_k, k_begin, k_end, k_sequences = (keep_q, q_begin, q_end, sequences) if cu_seqlens_k is None else \
+        row_bounds(cu_seqlens_k, device)
+    if k_sequences != sequences:
+        raise ConfigError(f"{sequences} sequences of queries, {k_sequences} of keys")
+    keys, kv_heads = key.shape[:2]
+    if cu_seqlens_k is None and keys != tokens:
+        raise ConfigError(f"{keys} keys for {tokens} queries need cu_seqlens_k")
+    fill = out is None
+    if out is None:
+        out = torch.empty(kv_heads, keys, dtype=torch.float32, device=device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (kv_heads, keys) or out.device != device or \
+            (keys > 1 and out.stride(1) != 1) or (kv_heads > 1 and out.stride(0) < keys):
+        raise ConfigError(f"out must be fp32 [{kv_heads}, {keys}] with contiguous rows apart on {device}")
+    query, key = operand(query), operand(key)
+    max_q = tokens if max_seqlen is None else min(int(max_seqlen), tokens)
+    max_k = keys if max_seqlen_k is None else min(int(max_seqlen_k), keys)
+    if cu_seqlens_k is None and max_seqlen_k is None:
+        max_k = max_q
+    with _lib.on(device):
+        _lib.call(
+            "eco_attention_mass", query.data_ptr(), _lib.fmt(query.dtype), *strides_of(query), key.data_ptr(),
+            *strides_of(key), lse.data_ptr(), lse.stride(0) if q_heads > 1 else tokens, q_begin, q_end, k_begin, k_end,
+            sequences, tokens, keys, max_q, max_k, min(int(window or 0), 0x7fffffff), out.data_ptr(),
+            out.stride(0) if kv_heads > 1 else keys, int(fill), q_heads, kv_heads, head_dim,
+            float(1 / math.sqrt(head_dim) if scale is None else scale), float(softcap or 0.0), _lib.stream_of(device))
+    return out

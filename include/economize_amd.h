@@ -463,6 +463,64 @@ int eco_kivi_packed_decode(const void* q, int32_t q_format, int64_t sq_b, int64_
                            int32_t kv_heads, int32_t keys, int32_t head_dim, int32_t value_dim, float scale,
                            float softcap, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- packed prompts and caches held at a budget -------------------------------------------------------------------
+ * Rows of sequence s: queries [q_begin[s], q_end[s]) and keys [k_begin[s], k_end[s]), int32 on the device, in order and
+ * apart (with cu_seqlens: begin = cu, end = cu + 1). Bounds are clamped to the rows there are. Query i of a sequence of nq
+ * queries and nk keys sees its keys j <= i + nk - nq. Tensors are bf16 or fp16, head dims 64, 128 and 256, channel stride
+ * 1, other strides in elements, multiples of 16 bytes from 0 to below 2^24. max_queries and max_keys are the longest
+ * sequence (they size the launch; longer ones are still computed whole). scale must be positive, softcap 0 means none.
+ * The reference has no counterpart: its evictions come as finished GatheredKV entries (attention/gathered.py:39-64). */
+
+/* Causal attention of every sequence's queries over its own keys: out [q_rows, Hq, D] and lse [Hq, sl_h] (optional, fp32:
+ * the logarithm of the softmax denominator, sinks [Hq] included). A query that sees no key gives 0 and lse -inf (its
+ * sink's logit with sinks). Rows of no sequence: 0 and -inf with fill, else left as they are. The workspace (optional
+ * where its size is 0) holds the parts of rows whose keys are cut. */
+size_t eco_prompt_attention_workspace_size(int32_t sequences, int32_t max_queries, int32_t max_keys, int32_t q_heads,
+                                           int32_t kv_heads, int32_t head_dim);
+int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, const void* v,
+                         int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h, const int32_t* q_begin,
+                         const int32_t* q_end, const int32_t* k_begin, const int32_t* k_end, int32_t sequences,
+                         int64_t q_rows, int64_t k_rows, int32_t max_queries, int32_t max_keys, const float* sinks,
+                         void* out, int64_t so_t, int64_t so_h, float* lse, int64_t sl_h, int32_t fill, int32_t q_heads,
+                         int32_t kv_heads, int32_t head_dim, float scale, float softcap, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* The attention weight every key received: mass[h, j] (fp32 [Hkv, sm_h]) = the sum over the queries that see key j (with
+ * window > 0 the last `window` of its sequence) and the query heads of KV head h of exp(score - lse). Keys of no
+ * sequence: 0 with fill, else left as they are. */
+int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t,
+                       int64_t sk_h, const float* lse, int64_t sl_h, const int32_t* q_begin, const int32_t* q_end,
+                       const int32_t* k_begin, const int32_t* k_end, int32_t sequences, int64_t q_rows, int64_t k_rows,
+                       int32_t max_queries, int32_t max_keys, int32_t window, float* mass, int64_t sm_h, int32_t fill,
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap, void* stream);
+
+/* A cache held at a budget of `slots` per row and KV head: keys / values [B, Hkv, slots, D], score fp32 and position
+ * int32 [B, Hkv, slots], count int32 [B, Hkv] filled slots, length int32 [B] tokens seen, all contiguous. The first
+ * `first` and the newest `recent` tokens are never evicted.
+ *
+ * Fills it from packed prompts, row b from key rows [begin[b], end[b]): of its n tokens every KV head keeps all if they
+ * fit, else the first, the newest and those of greatest mass [Hkv, sm_h] among the rest (equal: the lower index; a NaN is
+ * the least), in token order. Slots past the count are left as they are. max_tokens bounds nothing but the launch. */
+int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
+                     const float* mass, int64_t sm_h, const int32_t* begin, const int32_t* end, int64_t rows,
+                     int32_t max_tokens, void* keys, void* values, float* score, int32_t* position, int32_t* count,
+                     int32_t* length, int32_t batch, int32_t kv_heads, int32_t slots, int32_t head_dim, int32_t recent,
+                     int32_t first, void* stream);
+
+/* One decode step over it: the new token k / v [B, Hkv, D] at position length[b] takes slot count[b, h], or, when all are
+ * filled, the slot of least score whose position lies in [first, length[b] - recent] (equal: the lower slot; a NaN is
+ * the least); q [B, Hq, D] attends over the filled slots (out [B, Hq, D]); every filled slot's score grows by its weight
+ * summed over the query heads of its KV head (the new one's from 0); count and length advance. At most 64 query heads per
+ * KV head. The workspace need not be cleared. */
+size_t eco_heavy_hitter_workspace_size(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t slots,
+                                       int32_t head_dim);
+int eco_heavy_hitter_decode(const void* q, int32_t format, int64_t sq_b, int64_t sq_h, const void* k, const void* v,
+                            int64_t sk_b, int64_t sk_h, int64_t sv_b, int64_t sv_h, const float* sinks, void* keys,
+                            void* values, float* score, int32_t* position, int32_t* count, int32_t* length, void* out,
+                            int64_t so_b, int64_t so_h, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t slots,
+                            int32_t head_dim, int32_t recent, int32_t first, float scale, float softcap,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
