@@ -15,6 +15,9 @@ reasons, ``kernel_calls`` / ``kernel_usage`` / ``usage_summary``, the registrati
   attached (an eviction's compacted prompt entries), over the compact entries and the dense tail (path
   ``"kernel_gathered"``); with :class:`~economize_amd.quest.QuestPages` attached, over the selected pages and the
   dense tail (path ``"kernel_quest"``).
+* A key that carries a pass over a cache held at a budget (:class:`economize_amd.hf.HeavyHitterPass`) runs on its kernels
+  whatever its length (path ``"kernel_heavy_hitter"``): a prompt's attention, its keys' weights and their eviction, or
+  decode steps. It cannot fall back, since evicted tokens are gone; what the kernels do not take is refused.
 * Everything else falls back per call to transformers' ``sdpa`` (a paged cache's K/V materialized by the gather
   kernels first, fp8 K/V upcast to the query's dtype, Quest's unselected pages hidden in the mask as the reference's
   fallback hides them, interface.py:216-222), or to the model's eager function when the call has sinks or asks for
@@ -49,8 +52,8 @@ NAME = "economize"
 #: Longest query (tokens per row) the kernels take; longer ones (prefill) fall back to ``sdpa``.
 MAX_QUERIES = 64
 #: Packed formats the ``"economize"`` kernel reads (the reference's set, interface.py:70, plus the paged fp8 / bf16
-#: cache).
-PACKED_FORMATS = frozenset({"kivi", "gathered", "quest", "fp8", "bf16"})
+#: cache and the cache held at a budget).
+PACKED_FORMATS = frozenset({"kivi", "gathered", "quest", "fp8", "bf16", "heavy_hitter"})
 
 _DOT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -262,6 +265,23 @@ def _fallback_reason(module, query: torch.Tensor, key, attention_mask, dropout: 
     return None
 
 
+def _budget_refusal(module, query: torch.Tensor, dropout: float, is_causal: bool | None, kwargs: dict) -> str | None:
+    """Why a call over a cache held at a budget cannot run, or ``None`` when it can (its shapes, dtypes and mask are
+    checked by the pass itself)."""
+    if not query.is_cuda:
+        return "cpu"
+    if dropout > 0.0 and module is not None and module.training:
+        return "dropout"
+    sinks = _sinks(kwargs)
+    if sinks is not None and (not torch.is_tensor(sinks) or sinks.numel() != query.shape[1]):
+        return "sinks"
+    if kwargs.get("output_attentions", False):
+        return "output_attentions"
+    if is_causal is False and query.shape[2] > 1:
+        return "not_causal"
+    return None
+
+
 def _eager_function(module, kwargs: dict):
     """The model's own ``eager_attention_forward`` when the call needs it (sinks, attention weights), which ``sdpa``
     does not compute (interface.py:194-203)."""
@@ -322,12 +342,20 @@ def economize_attention_forward(module: torch.nn.Module | None, query: torch.Ten
     gathered = dense_packed if getattr(dense_packed, "format", None) == "gathered" else None
     layer = getattr(module, "layer_idx", None)
     queries = query.shape[2]
+    scale = query.shape[-1] ** -0.5 if scaling is None else scaling
+    if getattr(handle, "format", None) == "heavy_hitter":
+        reason = _budget_refusal(module, query, dropout, is_causal, kwargs)
+        if reason is not None:
+            raise ConfigError(f"attention over a heavy-hitter cache cannot fall back ({reason})")
+        out = handle.attend(query, key, value, attention_mask, scale, kwargs.get("softcap"), _sinks(kwargs))
+        _calls["kernel"] += 1
+        _usage[(layer, queries, "kernel_heavy_hitter", "")] += 1
+        return out, None
     reason = _fallback_reason(module, query, key, attention_mask, dropout, kwargs, paged, gathered)
     if reason is not None:
         if isinstance(key, PagedKV):
             raise ConfigError(f"a bare PagedKV handle cannot fall back ({reason}); attach it to dense stand-ins")
         return _fallback(module, query, key, value, attention_mask, dropout, scaling, is_causal, reason, kwargs)
-    scale = query.shape[-1] ** -0.5 if scaling is None else scaling
     softcap = kwargs.get("softcap")
     sinks = _sinks(kwargs)
     if paged is not None:
@@ -350,7 +378,7 @@ def economize_attention_forward(module: torch.nn.Module | None, query: torch.Ten
 ATTENTION_KERNELS.register(NAME, AttentionKernel(
     family="sdpa", forward=economize_attention_forward,
     description="MI355X decode attention: dense bf16/fp16/fp32/fp8 K/V with masks, paged fp8/bf16 and KIVI caches, "
-                "Quest pages",
+                "Quest pages, caches held at a budget",
     fp8_kv=True, packed_kv=PACKED_FORMATS, structured_masks=False,
 ))
 

@@ -25,6 +25,9 @@ for the techniques of this path:
   bounds kept incrementally). ``done[b]`` = committed full pages before the pass; a decoding query of a covered layer
   reads the selected pages and the tail (quest/technique.py:116-259), and a layer whose attached pages no attention
   function read raises when it is written next (quest/technique.py:174-182).
+* ``HeavyHitterConfig``: a cache of at most ``budget`` tokens per row and KV head (:class:`HeavyHitterLayer`). The first
+  pass attends over its own K/V on the packed prompt kernel and leaves the tokens of greatest attention weight; every
+  later token takes the slot of least weight. This package's own (the reference declares no eviction).
 
 A layer of no technique keeps dense K/V (transformers' ``DynamicLayer``) and attends on the dense kernel.
 
@@ -43,16 +46,18 @@ from transformers.cache_utils import Cache, CacheLayerMixin, DynamicLayer
 
 from .attention import MAX_QUERIES, NAME, PagedKV, install
 from .errors import ConfigError, IncompatibleTechniquesError
+from .eviction import HeavyHitterCache, evict_prompt, heavy_hitter_attention
 from .fp8 import calibrate_kv_absmax, fp8_encode, static_scales
 from .kivi import KIVI_PAGE, PagedKIVICache, kivi_append, kivi_commit, kivi_fake_quantize, kivi_quantize
 from .packed import attach_packed, stand_in
 from .paged import PAGE, PagedKVCache, paged_append
+from .prompt import attention_mass, prompt_attention
 from .quest import QuestPages, QuestState, bounds_dtype, page_bounds
-from .techniques import (FP8KVConfig, FusedFP8KVConfig, FusedKIVIConfig, KIVIConfig, QuestConfig, Technique,
-                         attn_implementation, head_dim_of, technique_for)
+from .techniques import (FP8KVConfig, FusedFP8KVConfig, FusedKIVIConfig, HeavyHitterConfig, KIVIConfig, QuestConfig,
+                         Technique, attn_implementation, head_dim_of, technique_for)
 
-__all__ = ["DenseFP8Layer", "DenseQuestLayer", "EconomizeCache", "EconomizedModel", "FusedKIVIDenseLayer", "KIVILayer",
-           "PackedKIVILayer", "PagedLayer", "SimulatedKIVILayer", "apply"]
+__all__ = ["DenseFP8Layer", "DenseQuestLayer", "EconomizeCache", "EconomizedModel", "FusedKIVIDenseLayer",
+           "HeavyHitterLayer", "HeavyHitterPass", "KIVILayer", "PackedKIVILayer", "PagedLayer", "SimulatedKIVILayer", "apply"]
 
 
 class _PagedBase(CacheLayerMixin):
@@ -853,6 +858,171 @@ class PackedKIVILayer(CacheLayerMixin):
             self.store.overflow.zero_()
 
 
+@dataclass
+class HeavyHitterPass:
+    """What one pass of a :class:`HeavyHitterLayer` attends over (the handle of format ``"heavy_hitter"``): the prompt's own
+    K/V, which it evicts from when it has attended, or the new tokens' K/V, which enter the cache one by one."""
+
+    layer: HeavyHitterLayer
+    keys: torch.Tensor  # [B, Hkv, T, D], the pass's own
+    values: torch.Tensor
+    prompt: bool
+    format: str = "heavy_hitter"
+
+    def attend(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, mask: torch.Tensor | None,
+               scale: float, softcap: float | None = None, sinks: torch.Tensor | None = None) -> torch.Tensor:
+        layer, cache = self.layer, self.layer.cache
+        layer._take(self)
+        batch, q_heads, tokens, dim = query.shape
+        if self.prompt:
+            pads = layer._prompt_padding(mask, batch, tokens)
+            q, k, v = (x.transpose(1, 2).reshape(batch * tokens, x.shape[1], dim)
+                       for x in (query, self.keys, self.values))
+            begin = torch.arange(0, batch * tokens, tokens, dtype=torch.int32, device=query.device)
+            rows = (begin if pads is None else begin + pads, begin + tokens)
+            out, lse = prompt_attention(q, k, v, rows, tokens, scale, softcap=softcap, sinks=sinks, return_lse=True)
+            mass = attention_mass(q, k, lse, rows, tokens, scale, window=layer.config.window, softcap=softcap)
+            evict_prompt(cache, k, v, mass, rows, tokens)
+            return out.view(batch, tokens, q_heads, dim)
+        layer._check_mask(mask, batch, tokens)
+        out = torch.empty(batch, tokens, q_heads, dim, dtype=query.dtype, device=query.device)
+        for t in range(tokens):
+            heavy_hitter_attention(cache, query[:, :, t], self.keys[:, :, t], self.values[:, :, t], scale, softcap,
+                                   sinks, out=out[:, t])
+        return out
+
+    def materialize(self) -> tuple[torch.Tensor, torch.Tensor]:
+        if self.prompt:
+            return self.keys, self.values
+        raise IncompatibleTechniquesError("evicted tokens are gone: a heavy-hitter cache is read by "
+                                          "attn_implementation='economize' only")
+
+
+class HeavyHitterLayer(CacheLayerMixin, _UnreadCheck):
+    """One layer's K/V held at ``config.budget`` tokens per row and KV head (:class:`~economize_amd.eviction.
+    HeavyHitterCache`). The first pass is the prompt: it attends over its own K/V (packed prompt attention), its keys' attention
+    weights are summed, and the heaviest tokens stay. Every later token takes the slot of least weight and adds the weights
+    it gives; a later pass of many tokens runs them one after the other. Counts and positions live on the device; a decoding
+    step without a mask can be captured in a graph.
+
+    A mask must be the causal one, over a left-padded batch or a full one (checked on the device, which waits for it; a
+    captured pass takes none); padding is not kept and counts as no token."""
+
+    is_sliding = False
+    is_compileable = False
+    supports_early_init = False
+
+    def __init__(self, config: HeavyHitterConfig, layer: int = 0) -> None:
+        super().__init__()
+        self.config = config
+        self.cache: HeavyHitterCache | None = None
+        self.length = 0
+        self._pads: torch.Tensor | None = None  # int32 [B] padding columns in front of every row
+        self._pending: HeavyHitterPass | None = None
+        self._init_unread(layer)
+
+    def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
+        batch, heads, _, dim = key_states.shape
+        c = self.config
+        self.cache = HeavyHitterCache.empty(batch, heads, dim, c.budget, key_states.dtype, key_states.device, c.recent,
+                                            c.first)
+        self.is_initialized = True
+
+    def get_seq_length(self) -> int:
+        return self.length
+
+    def get_mask_sizes(self, query_length: int) -> tuple[int, int]:
+        return self.length + query_length, 0
+
+    def get_max_length(self) -> int:
+        return -1
+
+    def allocated_bytes(self) -> int:
+        """Bytes the layer holds on the device."""
+        c = self.cache
+        return 0 if c is None else sum(t.numel() * t.element_size() for t in (c.keys, c.values, c.score, c.position,
+                                                                              c.count, c.length))
+
+    def _take(self, handle: HeavyHitterPass) -> None:
+        """A pass is attended over once: it changes the cache."""
+        if self._pending is not handle:
+            raise IncompatibleTechniquesError(f"heavy_hitter's pass of cache layer {self.layer_idx} was attended over "
+                                              "already, or a newer one has begun")
+        self._pending = None
+        self._read(self.layer_idx)
+
+    def _prompt_padding(self, mask: torch.Tensor | None, batch: int, tokens: int) -> torch.Tensor | None:
+        if mask is None:
+            return None
+        self._boolean(mask, batch, tokens)
+        pads = (~mask[:, 0, -1, :tokens]).sum(-1).clamp(max=tokens - 1).to(torch.int32).expand(batch).contiguous()
+        self._pads = pads
+        self._check_mask(mask, batch, tokens)
+        return pads
+
+    def _boolean(self, mask: torch.Tensor, batch: int, tokens: int) -> None:
+        if mask.dtype != torch.bool or mask.dim() != 4 or mask.shape[0] not in (1, batch) or mask.shape[1] != 1 or \
+                mask.shape[2] != tokens or mask.shape[3] < self.length:
+            raise ConfigError(f"a heavy-hitter cache takes a boolean mask [B or 1, 1, {tokens}, >= {self.length}], got "
+                              f"{mask.dtype} {tuple(mask.shape)}")
+        if torch.cuda.is_current_stream_capturing():
+            raise ConfigError("a captured pass over a heavy-hitter cache takes no mask (checking it waits for the device)")
+
+    def _check_mask(self, mask: torch.Tensor | None, batch: int, tokens: int) -> None:
+        """The mask hides the padding in front and what comes after each query, and nothing else."""
+        if mask is None:
+            if self._pads is not None and not torch.cuda.is_current_stream_capturing() and bool(self._pads.any()):
+                raise ConfigError("a left-padded heavy-hitter cache needs its mask in every pass")
+            return
+        self._boolean(mask, batch, tokens)
+        pads = torch.zeros(batch, dtype=torch.int32, device=mask.device) if self._pads is None else self._pads
+        j = torch.arange(self.length, device=mask.device)
+        i = torch.arange(self.length - tokens, self.length, device=mask.device)
+        real = i[None, :, None] >= pads[:, None, None]
+        want = (j >= pads[:, None, None]) & (j <= i[None, :, None])
+        if not bool(((mask[:, 0, :, : self.length] == want) | ~real).all()):
+            raise ConfigError("a heavy-hitter cache takes the causal mask of a left-padded or full batch only: evicted "
+                              "tokens cannot be masked one by one")
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+        if not self.is_initialized:
+            self.lazy_initialization(key_states, value_states)
+        if self._unread:
+            self._unread = False
+            raise IncompatibleTechniquesError(
+                f"heavy_hitter's pass of cache layer {self.layer_idx} was not attended over: run the model with "
+                "attn_implementation='economize' (economize_amd.attention.install()) and let no technique copy the keys")
+        prompt = self.length == 0
+        tokens = key_states.shape[2]
+        self.length += tokens
+        self._pending = HeavyHitterPass(self, key_states, value_states, prompt)
+        self._attached()
+        if prompt:
+            return attach_packed(key_states, self._pending), value_states
+        batch, heads, _, dim = key_states.shape
+        shape = (batch, heads, self.length, dim)
+        keys = stand_in(shape, key_states.dtype, key_states.device)
+        return attach_packed(keys, self._pending), stand_in(shape, key_states.dtype, key_states.device)
+
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        """Rows by ``beam_idx`` (beam search)."""
+        if self.cache is None:
+            return
+        c, at = self.cache, beam_idx.to(self.cache.keys.device)
+        for name in ("keys", "values", "score", "position", "count", "length"):
+            setattr(c, name, getattr(c, name).index_select(0, at))
+        if self._pads is not None:
+            self._pads = self._pads.index_select(0, at)
+
+    def reset(self) -> None:
+        self.length = 0
+        self._pads = self._pending = None
+        self._unread = False
+        if self.cache is not None:
+            self.cache.reset()
+
+
 class EconomizeCache(Cache):
     """transformers ``past_key_values`` whose layers are the techniques' paged caches (dense ``DynamicLayer`` for a
     layer no technique covers)."""
@@ -923,7 +1093,8 @@ class EconomizedModel:
             technique = self.technique_of(index + 1)
             cfg = technique.config if technique is not None else None
             if static:
-                if isinstance(cfg, KIVIConfig) or (isinstance(cfg, FP8KVConfig) and not self.paged_fp8(cfg)):
+                if isinstance(cfg, (KIVIConfig, HeavyHitterConfig)) or (isinstance(cfg, FP8KVConfig) and
+                                                                        not self.paged_fp8(cfg)):
                     raise ConfigError(f"a static cache holds layers of no technique, paged fp8 and Quest, not "
                                       f"{type(cfg).__name__} on layer {index + 1}")
                 fp8 = cfg.dtype if isinstance(cfg, FP8KVConfig) else None
@@ -931,7 +1102,9 @@ class EconomizedModel:
                 layers.append(PagedLayer(max_length, fp8, quest, scales=self.scales.get(index), layer=index,
                                          static=True))
                 continue
-            if isinstance(cfg, KIVIConfig):
+            if isinstance(cfg, HeavyHitterConfig):
+                layers.append(HeavyHitterLayer(cfg, layer=index))
+            elif isinstance(cfg, KIVIConfig):
                 kind = cfg.layer_kind(self.model)
                 layer_class = {"paged": KIVILayer, "packed": PackedKIVILayer, "fused": FusedKIVIDenseLayer,
                                "simulated": SimulatedKIVILayer}[kind]

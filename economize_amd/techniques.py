@@ -6,6 +6,8 @@
 * :class:`KIVIConfig` / :class:`FusedKIVIConfig` follow techniques/kv_quant/kivi.py:53-107 and
   techniques/kv_kivi_fused/fused.py:30-51.
 * :class:`QuestConfig` follows techniques/quest/technique.py:45-115.
+* :class:`HeavyHitterConfig` is this package's own: the reference reads evicted caches (attention/gathered.py:39-64) but
+  declares no eviction.
 * :func:`register_technique`, :data:`TECHNIQUES` and :func:`technique_for` follow core/technique.py:345-375.
 
 A technique makes the paged layer cache its configuration describes (:meth:`Technique.make_cache`); the caches and
@@ -23,8 +25,8 @@ import torch
 from .errors import ConfigError, IncompatibleTechniquesError
 
 __all__ = [
-    "FP8KVConfig", "FusedFP8KVConfig", "FusedKIVIConfig", "KIVIConfig", "QuestConfig", "Registry", "TECHNIQUES",
-    "Technique", "TechniqueConfig", "register_technique", "technique_for",
+    "FP8KVConfig", "FusedFP8KVConfig", "FusedKIVIConfig", "HeavyHitterConfig", "KIVIConfig", "QuestConfig", "Registry",
+    "TECHNIQUES", "Technique", "TechniqueConfig", "register_technique", "technique_for",
 ]
 
 FP8_FORMATS: dict[str, torch.dtype] = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
@@ -364,6 +366,49 @@ class QuestConfig(TechniqueConfig):
                       "its pages", None)
 
 
+@dataclass(frozen=True)
+class HeavyHitterConfig(TechniqueConfig):
+    """A cache of at most ``budget`` tokens per row and KV head, those that received the most attention weight.
+
+    Attributes:
+        budget: Tokens every KV head keeps.
+        recent: The newest tokens, always kept.
+        first: The first tokens of a row, always kept.
+        window: Weigh a prompt's tokens by its last ``window`` queries only (``None``: by all).
+        layers: 1-indexed layers the technique acts on (empty: every layer).
+    """
+
+    technique: ClassVar[str] = "heavy_hitter"
+    budget: int = 1024
+    recent: int = 128
+    first: int = 4
+    window: int | None = None
+    layers: tuple[int, ...] = ()
+
+    def __post_init__(self) -> None:
+        _positive("budget", self.budget)
+        _positive("recent", self.recent)
+        if isinstance(self.first, bool) or not isinstance(self.first, Integral) or self.first < 0:
+            raise ConfigError(f"first must be a non-negative integer, got {self.first!r}")
+        if self.recent + self.first > self.budget:
+            raise ConfigError(f"recent ({self.recent}) and first ({self.first}) exceed the budget ({self.budget})")
+        if self.window is not None:
+            _positive("window", self.window)
+        _layers(self.layers)
+
+    def validate(self, adapter) -> None:
+        """Refuses models whose attention the kernels do not take (bf16 or fp16, head dims 64, 128 and 256) and
+        attention implementations that do not read the cache."""
+        from .attention import accepts_packed_kv
+
+        _head_dims(self.technique, adapter, (64, 128, 256))
+        dtype = model_dtype(adapter)
+        if dtype is not None and dtype not in (torch.bfloat16, torch.float16):
+            raise ConfigError(f"{self.technique}: the MI355X kernels take bf16 and fp16 models, not {dtype}")
+        _needs_kernel(self.technique, attn_implementation(adapter),
+                      lambda name: accepts_packed_kv(name, self.technique), "a heavy-hitter cache", None)
+
+
 # ---- techniques -----------------------------------------------------------------------------------------------
 
 TECHNIQUES: Registry = Registry("technique")
@@ -380,6 +425,8 @@ def technique_for(config) -> Technique:
     technique = getattr(type(config), "technique", None)
     if technique is None:
         raise ConfigError(f"{type(config).__name__} is not a technique configuration")
+    if isinstance(config, HeavyHitterConfig):  # (the registry holds the techniques the reference declares)
+        return HeavyHitterTechnique(config)
     return TECHNIQUES.get_entry(technique)(config)
 
 
@@ -458,3 +505,15 @@ class QuestTechnique(Technique):
         shape = (batch, kv_heads, max_pages, head_dim)
         return (torch.zeros(shape, dtype=torch.bfloat16, device=device),
                 torch.zeros(shape, dtype=torch.bfloat16, device=device))
+
+
+class HeavyHitterTechnique(Technique):
+    config_class = HeavyHitterConfig
+    packed_format = "heavy_hitter"
+
+    def make_cache(self, *, batch: int, kv_heads: int, head_dim: int, device, dtype: torch.dtype = torch.bfloat16, **_):
+        """An empty :class:`~economize_amd.eviction.HeavyHitterCache`."""
+        from .eviction import HeavyHitterCache
+
+        c = self.config
+        return HeavyHitterCache.empty(batch, kv_heads, head_dim, c.budget, dtype, device, c.recent, c.first)
