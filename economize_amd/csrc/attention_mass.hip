@@ -22,7 +22,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
     __shared__ __align__(16) uint8_t lds[2][Tile<D>::BYTES];
     __shared__ __align__(16) float stat[2][64];
 
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
     const int pairs = p.rows.sequences * p.kv_heads;
     const int id = blockIdx.x;
     if (id >= pairs * p.tiles) {  // the last workgroups: keys of no sequence
@@ -108,20 +108,27 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
                         ls[i] = *reinterpret_cast<const float4*>(&stat[buf][32 * b + 8 * i + 4 * half]);
 #pragma unroll
                     for (int u = 0; u < KT; ++u) {
-                        const int key = key0 + 32 * u + col;
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const float4 four = ls[r >> 2];
                             const float l = (r & 3) == 0 ? four.x : (r & 3) == 1 ? four.y : (r & 3) == 2 ? four.z : four.w;
                             float y = x[u][r];
                             if constexpr (CAP) y = soft_cap_log2(y * p.scale, p.softcap, 1.0f / p.softcap);
-                            y = __builtin_fmaf(y, cc, -l);
-                            if (masked) {
-                                const int i = i0 + 32 * b + 8 * (r >> 2) + 4 * half + (r & 3);
-                                if (key > i + offset || i >= seq.nq) y = -INFINITY;
-                            }
-                            sum[u] += __builtin_amdgcn_exp2f(y);
+                            x[u][r] = __builtin_fmaf(y, cc, -l);
                         }
+                        if (masked) {
+                            asm volatile("" ::: );  // (a branch of its own: as selects the masks would cost every tile)
+                            const int key = key0 + 32 * u + col;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const int i = i0 + 32 * b + 8 * (r >> 2) + 4 * half + (r & 3);
+                                if (key > i + offset || i >= seq.nq) x[u][r] = -INFINITY;
+                            }
+                        }
+                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // short sums first: their rounding stays small
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) part[r & 3] += __builtin_amdgcn_exp2f(x[u][r]);
+                        sum[u] += (part[0] + part[1]) + (part[2] + part[3]);
                     }
                 }
             }

@@ -42,7 +42,7 @@ struct HeavyParams {
     int splits, span;  // parts a row's slots are cut into, slots of a part
     float scale, softcap;
     float* logits;   // workspace: [B, Hkv, G, C]
-    float* partial;  // [B, Hkv, splits, 16 NB, D + 2]
+    float* partial;  // [B, Hkv, splits, G, D + 2]
     int32_t* plan;   // [B, Hkv, 4]: the slot written, filled slots, position
 };
 

@@ -9,6 +9,7 @@
 // heavy_merge_kernel: the parts' join, and the weights from the scores kept, added to the slots' scores. Every sum has a
 // fixed order: no atomics.
 
+#include <cstdlib>
 #include "eviction.hpp"
 
 namespace eco {
@@ -50,11 +51,23 @@ __device__ __forceinline__ int choose_slot(const BudgetCache& c, int bh, int fil
     const float* score = c.score + static_cast<int64_t>(bh) * c.slots;
     const int32_t* position = c.position + static_cast<int64_t>(bh) * c.slots;
     uint64_t best = ~0ull;
-    for (int i = threadIdx.x; i < c.slots; i += THREADS) {
-        const int pos = position[i];
-        const bool free = pos >= c.first && pos <= token - c.recent;
-        const uint64_t key = static_cast<uint64_t>(free ? score_rank(score[i]) : 0xFFFFFFFFu) << 32 | static_cast<uint32_t>(i);
-        best = key < best ? key : best;
+    constexpr int AT_ONCE = 8;  // slots per thread whose loads are in flight together
+    for (int i0 = threadIdx.x; i0 < c.slots; i0 += AT_ONCE * THREADS) {
+        int pos[AT_ONCE];
+        float sc[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = i0 + j * THREADS < c.slots ? i0 + j * THREADS : c.slots - 1;
+            pos[j] = position[i];
+            sc[j] = score[i];
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int i = i0 + j * THREADS < c.slots ? i0 + j * THREADS : c.slots - 1;
+            const bool free = pos[j] >= c.first && pos[j] <= token - c.recent;
+            const uint64_t key = static_cast<uint64_t>(free ? score_rank(sc[j]) : 0xFFFFFFFFu) << 32 | static_cast<uint32_t>(i);
+            best = key < best ? key : best;
+        }
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -68,23 +81,67 @@ __device__ __forceinline__ int choose_slot(const BudgetCache& c, int bh, int fil
     return static_cast<int>(static_cast<uint32_t>(best));
 }
 
+// 32 slots of one wave in LDS, in chunks of 16 bytes; the swizzles spread the rows of one fragment read (16 rows of 16
+// bytes per 16 lanes; transposed: 8 rows of 32 bytes per 32 lanes) over all banks.
+template <int D>
+struct SlotTile {
+    static constexpr int CHUNKS = D / 8;
+    static constexpr int BYTES = 32 * D * 2;
+    static constexpr int N = 32 * CHUNKS / 64;  // chunks per lane
+    static __device__ __forceinline__ int key_at(int row, int chunk) {
+        const int c = CHUNKS == 8 ? chunk ^ ((row >> 1) & 7) : chunk ^ (row & 15);
+        return row * (D * 2) + c * 16;
+    }
+    static __device__ __forceinline__ int value_at(int row, int chunk) {
+        const int c = CHUNKS == 8 ? chunk ^ (((row >> 1) & 3) << 1) : chunk ^ ((row & 7) << 1);
+        return row * (D * 2) + c * 16;
+    }
+};
+
 template <int D, int FMT>
-__global__ __launch_bounds__(THREADS, 2) void heavy_attend_kernel(HeavyParams p) {
-    constexpr int KS = D / 32;     // 32-channel steps of the first product
-    constexpr int DT = D / 16;     // 16-channel blocks of the output
-    constexpr int PITCH = D * 2 + 16;
-    constexpr int CH = D / 8 / 2;  // 16-byte chunks of 32 value rows per lane
-    __shared__ __align__(16) uint8_t vlds[WAVES][32 * PITCH];
+__global__ __launch_bounds__(THREADS, (D == 256 ? 1 : 2)) void heavy_attend_kernel(HeavyParams p) {
+    typedef SlotTile<D> T;
+    constexpr int KS = D / 32;  // 32-channel steps of the first product
+    constexpr int DT = D / 16;  // 16-channel blocks of the output
+    __shared__ __align__(16) uint8_t tiles[WAVES][2][T::BYTES];
     __shared__ uint64_t scratch[WAVES];
     __shared__ float wm[WAVES][16], wl[WAVES][16];
 
     const BudgetCache& c = p.cache;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, grp = lane >> 4;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, grp = lane >> 4;
     const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
     const int split = blockIdx.y, block = blockIdx.z;
+    uint16_t* keys = c.keys + static_cast<int64_t>(bh) * c.slots * D;
+    uint16_t* values = c.values + static_cast<int64_t>(bh) * c.slots * D;
+    const int s0 = split * p.span, end = s0 + p.span < c.slots ? s0 + p.span : c.slots;
+
+    // A tile's slots on their way; those past the row's last slot are read from it (any slot may be read: only what is
+    // filled is used).
+    uint4 kr[T::N], vr[T::N];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < T::N; ++i) {
+            const int at = lane + 64 * i;
+            int slot = k0 + at / T::CHUNKS;
+            slot = slot < end ? slot : end - 1;
+            kr[i] = stream_load16(keys + static_cast<int64_t>(slot) * D + at % T::CHUNKS * 8);
+            vr[i] = stream_load16(values + static_cast<int64_t>(slot) * D + at % T::CHUNKS * 8);
+        }
+    };
+    const int first_slot = s0 + 32 * wave;
+    if (first_slot < end) load(first_slot);  // before anything of the row is known: its slot is chosen meanwhile
+
     int filled = c.count[bh];
     filled = filled < 0 ? 0 : (filled > c.slots ? c.slots : filled);
     const int token = c.length[b];
+    const int head = block * 16 + col;
+    const bool head_there = head < p.groups;
+    const uint16_t* qp = p.q + b * p.sq_b + (h * p.groups + (head_there ? head : p.groups - 1)) * p.sq_h + grp * 8;
+    uint4 qf[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) qf[i] = *reinterpret_cast<const uint4*>(qp + 32 * i);
+    const uint16_t* new_k = p.k + b * p.sk_b + h * p.sk_h;
+    const uint16_t* new_v = p.v + b * p.sv_b + h * p.sv_h;
     const int to = choose_slot(c, bh, filled, token, scratch);
     const int n = filled < c.slots ? filled + 1 : c.slots;
     if (split == 0 && block == 0 && tid == 0) {
@@ -93,17 +150,7 @@ __global__ __launch_bounds__(THREADS, 2) void heavy_attend_kernel(HeavyParams p)
         plan[1] = n;
         plan[2] = token;
     }
-    const uint16_t* new_k = p.k + b * p.sk_b + h * p.sk_h;
-    const uint16_t* new_v = p.v + b * p.sv_b + h * p.sv_h;
-    uint16_t* keys = c.keys + static_cast<int64_t>(bh) * c.slots * D;
-    uint16_t* values = c.values + static_cast<int64_t>(bh) * c.slots * D;
-    const int s0 = split * p.span, s1 = s0 + p.span < n ? s0 + p.span : n;
-    const int head = block * 16 + col;
-    const bool head_there = head < p.groups;
-    const uint16_t* qp = p.q + b * p.sq_b + (h * p.groups + (head_there ? head : p.groups - 1)) * p.sq_h + grp * 8;
-    uint4 qf[KS];
-#pragma unroll
-    for (int i = 0; i < KS; ++i) qf[i] = *reinterpret_cast<const uint4*>(qp + 32 * i);
+    const int s1 = end < n ? end : n;
     float* logits = p.logits + (static_cast<int64_t>(bh) * p.groups + head) * c.slots;
 
     f32x4 acc[DT];
@@ -111,31 +158,28 @@ __global__ __launch_bounds__(THREADS, 2) void heavy_attend_kernel(HeavyParams p)
     for (int d = 0; d < DT; ++d) acc[d] = f32x4{};
     float m = NEVER, l = 0.0f;
     const float c2 = p.scale * kLog2e;
-    uint8_t* vl = vlds[wave];
-    for (int k0 = s0 + 32 * wave; k0 < s1; k0 += 32 * WAVES) {
-        uint4 kf[2][KS], vf[CH];
+    uint8_t *kl = tiles[wave][0], *vl = tiles[wave][1];
+    for (int k0 = first_slot; k0 < s1; k0 += 32 * WAVES) {
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            int slot = k0 + 16 * v + col;
-            slot = slot < s1 ? slot : s1 - 1;
-            const uint16_t* kp = (slot == to ? new_k : keys + static_cast<int64_t>(slot) * D) + grp * 8;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) kf[v][i] = *reinterpret_cast<const uint4*>(kp + 32 * i);
+        for (int i = 0; i < T::N; ++i) {
+            const int at = lane + 64 * i, row = at / T::CHUNKS, chunk = at % T::CHUNKS;
+            *reinterpret_cast<uint4*>(kl + T::key_at(row, chunk)) = kr[i];
+            // (a weight of 0 times what an unfilled slot holds must be 0)
+            *reinterpret_cast<uint4*>(vl + T::value_at(row, chunk)) = k0 + row < s1 ? vr[i] : make_uint4(0, 0, 0, 0);
         }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int at = lane + 64 * i, row = at / (D / 8), chunk = at % (D / 8);
-            int slot = k0 + row;
-            slot = slot < s1 ? slot : s1 - 1;
-            vf[i] = *reinterpret_cast<const uint4*>((slot == to ? new_v : values + static_cast<int64_t>(slot) * D) +
-                                                    chunk * 8);
+        if (k0 + 32 * WAVES < s1) load(k0 + 32 * WAVES);
+        __builtin_amdgcn_wave_barrier();
+        if (to >= k0 && to < k0 + 32 && lane < T::CHUNKS) {  // the new token over the one it replaces
+            *reinterpret_cast<uint4*>(kl + T::key_at(to - k0, lane)) = reinterpret_cast<const uint4*>(new_k)[lane];
+            *reinterpret_cast<uint4*>(vl + T::value_at(to - k0, lane)) = reinterpret_cast<const uint4*>(new_v)[lane];
         }
+        __builtin_amdgcn_wave_barrier();
         f32x4 x[2] = {f32x4{}, f32x4{}};
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            x[0] = mfma16<FMT>(kf[0][i], qf[i], x[0]);
-            x[1] = mfma16<FMT>(kf[1][i], qf[i], x[1]);
-        }
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+                x[v] = mfma16<FMT>(*reinterpret_cast<const uint4*>(kl + T::key_at(16 * v + col, 4 * i + grp)), qf[i], x[v]);
         float mx = NEVER;
 #pragma unroll
         for (int v = 0; v < 2; ++v)
@@ -171,12 +215,6 @@ __global__ __launch_bounds__(THREADS, 2) void heavy_attend_kernel(HeavyParams p)
             pw[2 * v + 1] = pair16<FMT>(e[2], e[3]);
         }
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int at = lane + 64 * i, row = at / (D / 8), chunk = at % (D / 8);
-            *reinterpret_cast<uint4*>(vl + row * PITCH + chunk * 16) = vf[i];
-        }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
         for (int d = 0; d < DT; ++d) {
             typedef short i16x4 __attribute__((ext_vector_type(4)));
             uint2 w[2];
@@ -184,7 +222,7 @@ __global__ __launch_bounds__(THREADS, 2) void heavy_attend_kernel(HeavyParams p)
             for (int v = 0; v < 2; ++v)
                 w[v] = __builtin_bit_cast(
                     uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(
-                               vl + (16 * v + 4 * grp + (col >> 2)) * PITCH + 32 * d + 8 * (col & 3))));
+                               vl + T::value_at(16 * v + 4 * grp + (col >> 2), 2 * d + ((col & 3) >> 1)) + 8 * (col & 1))));
             acc[d] = mfma16<FMT>(make_uint4(w[0].x, w[0].y, w[1].x, w[1].y), make_uint4(pw[0], pw[1], pw[2], pw[3]),
                                  acc[d]);
         }
@@ -192,6 +230,7 @@ __global__ __launch_bounds__(THREADS, 2) void heavy_attend_kernel(HeavyParams p)
     }
     // the new token's row, by the part that holds its slot
     if (to >= s0 && to < s1 && block == 0) {
+        __syncthreads();  // every wave's reads of the part are done
         for (int i = tid; i < D / 8; i += THREADS) {
             reinterpret_cast<uint4*>(keys + static_cast<int64_t>(to) * D)[i] = reinterpret_cast<const uint4*>(new_k)[i];
             reinterpret_cast<uint4*>(values + static_cast<int64_t>(to) * D)[i] = reinterpret_cast<const uint4*>(new_v)[i];
@@ -212,27 +251,26 @@ __global__ __launch_bounds__(THREADS, 2) void heavy_attend_kernel(HeavyParams p)
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) sum += wl[w][col] * __builtin_amdgcn_exp2f(wm[w][col] - top);
     const float a = __builtin_amdgcn_exp2f(m - top);
-    float* joined = reinterpret_cast<float*>(&vlds[0][0]);  // [16][D + 4]: the values in it are used up
+    float* joined = reinterpret_cast<float*>(&tiles[0][0][0]);  // [WAVES][16][D + 4]: the slots in it are used up
     constexpr int JP = D + 4;
-    static_assert(16 * JP * 4 <= WAVES * 32 * PITCH, "the join fits the value tiles");
-    for (int w = 0; w < WAVES; ++w) {  // in turn: a fixed order
-        __syncthreads();
-        if (w == wave) {
+    static_assert(WAVES * 16 * JP * 4 <= sizeof(tiles), "the join fits the tiles");
+    __syncthreads();
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float* at = joined + col * JP + 16 * d + 4 * grp + r;
-                    const float y = acc[d][r] * a;
-                    *at = w == 0 ? y : *at + y;
-                }
-        }
+    for (int d = 0; d < DT; ++d) {
+        float4 y = make_float4(acc[d][0] * a, acc[d][1] * a, acc[d][2] * a, acc[d][3] * a);
+        *reinterpret_cast<float4*>(joined + (wave * 16 + col) * JP + 16 * d + 4 * grp) = y;
     }
     __syncthreads();
-    const int heads = (p.groups + 15) / 16 * 16;
-    float* part = p.partial + ((static_cast<int64_t>(bh) * p.splits + split) * heads + block * 16) * (D + 2);
-    for (int i = tid; i < 16 * D; i += THREADS) part[(i / D) * (D + 2) + 2 + i % D] = joined[(i / D) * JP + i % D];
-    if (tid < 16) {
+    const int heads = p.groups - block * 16 < 16 ? p.groups - block * 16 : 16;
+    float* part = p.partial + ((static_cast<int64_t>(bh) * p.splits + split) * p.groups + block * 16) * (D + 2);
+    for (int i = tid; i < heads * D; i += THREADS) {
+        const int g = i / D, d = i % D;
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) y += joined[(w * 16 + g) * JP + d];
+        part[g * (D + 2) + 2 + d] = y;
+    }
+    if (tid < heads) {
         part[tid * (D + 2)] = top;
         part[tid * (D + 2) + 1] = sum;
     }
@@ -246,9 +284,8 @@ __global__ __launch_bounds__(THREADS) void heavy_merge_kernel(HeavyParams p) {
     const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
     const int32_t* plan = p.plan + 4 * static_cast<int64_t>(bh);
     const int to = plan[0], n = plan[1], token = plan[2];
-    const int heads = (p.groups + 15) / 16 * 16;
-    const float* part = p.partial + static_cast<int64_t>(bh) * p.splits * heads * (D + 2);
-    const int64_t step = static_cast<int64_t>(heads) * (D + 2);
+    const int64_t step = static_cast<int64_t>(p.groups) * (D + 2);
+    const float* part = p.partial + static_cast<int64_t>(bh) * p.splits * step;
     if (tid < p.groups) {
         float top = NEVER;
         for (int s = 0; s < p.splits; ++s) {
@@ -310,14 +347,15 @@ Plan make_plan(int batch, int q_heads, int kv_heads, int slots, int head_dim, in
     Plan r;
     const int groups = q_heads / kv_heads;
     const int64_t rows = static_cast<int64_t>(batch) * kv_heads;
-    int64_t splits = (2 * static_cast<int64_t>(cus) + rows - 1) / rows;
+    static const int per = getenv("ECO_HH") ? atoi(getenv("ECO_HH")) : 2;
+    int64_t splits = (per * static_cast<int64_t>(cus) + rows - 1) / rows;
     const int64_t most = (slots + 127) / 128;
     splits = splits > most ? most : splits;
     r.span = static_cast<int>(((slots + splits - 1) / splits + 127) / 128 * 128);
     r.splits = (slots + r.span - 1) / r.span;
     auto align = [](size_t x) { return (x + 255) / 256 * 256; };
     r.logits = align(sizeof(float) * rows * groups * slots);
-    r.partial = align(sizeof(float) * rows * r.splits * ceil_div(groups, 16) * 16 * (head_dim + 2));
+    r.partial = align(sizeof(float) * rows * r.splits * groups * (head_dim + 2));
     r.plan = align(sizeof(int32_t) * rows * 4);
     return r;
 }

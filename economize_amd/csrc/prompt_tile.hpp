@@ -129,4 +129,88 @@ struct TileLoad {
     }
 };
 
+// Every wave's copies have arrived and its LDS accesses are done, in all waves of the workgroup.
+__device__ __forceinline__ void tile_barrier() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_byte*)p));
+}
+
+__device__ __forceinline__ uint4 lds_read16(uint32_t at) {
+    return __builtin_bit_cast(
+        uint4, *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>((lds_byte*)static_cast<uintptr_t>(at)));
+}
+
+// ds_read_b64_tr_b16: the 16 lanes of a group name four rows of 16 elements, lane 4 k + q the eight bytes of row k's
+// elements 4 q .. 4 q + 3; lane i receives element i of the four rows.
+__device__ __forceinline__ uint2 lds_read_transposed(uint32_t at) {
+    typedef short i16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) i16x4*)static_cast<uintptr_t>(at)));
+}
+
+// Copies of 64-row tiles straight into LDS (buffer_load_dwordx4 ... lds: 64 lanes' 16 bytes in a row from the address in
+// M0), by 256 threads. A lane's place in LDS is fixed, so it fetches the chunk the swizzle puts there. Rows past the
+// sequence's end are outside the buffer resource. The copies of a tile complete at the workgroup's next tile_barrier.
+template <int D>
+struct TileCopy {
+    static constexpr int CHUNKS = D / 8, N = 64 * CHUNKS / 256, ROWS = 256 / CHUNKS;  // rows per instruction of 4 waves
+    static constexpr int KINDS = D == 256 ? 2 : 1;  // the swizzle repeats every 16 rows
+    uint32_t from[KINDS];
+    int wave;
+
+    __device__ __forceinline__ TileCopy(int tid, int64_t stride, bool keys) {
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+        for (int i = 0; i < KINDS; ++i) {
+            const int row = tid / CHUNKS + i * ROWS, at = tid % CHUNKS;
+            const int chunk = keys ? Tile<D>::key_chunk(row, at) : Tile<D>::value_chunk(row, at);
+            from[i] = static_cast<uint32_t>(tid / CHUNKS) * static_cast<uint32_t>(stride * 2) + chunk * 16u;
+        }
+    }
+
+    __device__ __forceinline__ void start(uint8_t* lds, const uint16_t* base, int64_t stride, int row0, int rows) const {
+        const int left = rows - row0;
+        const int n = left < 64 ? left : 64;
+        const uint32_t bytes = n <= 0 ? 0u : static_cast<uint32_t>((n - 1) * stride * 2 + D * 2);
+        const uint64_t at = reinterpret_cast<uint64_t>(base + static_cast<int64_t>(row0) * stride);
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        i32x4 rsrc;
+        rsrc[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(at));
+        rsrc[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32) & 0xFFFF);
+        rsrc[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
+        rsrc[3] = 0x00020000;
+        const uint32_t to = lds_address(lds) + wave * 1024u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + i * 4096u);
+            const uint32_t skip = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(i * ROWS) * static_cast<uint32_t>(stride * 2));
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                         :: "s"(m0), "v"(from[i % KINDS]), "s"(rsrc), "s"(skip) : "memory");
+        }
+    }
+};
+
+// Infinities and NaN of a tile of values in LDS to 0, by 256 threads; whether this thread found one.
+template <int D, int FMT>
+__device__ __forceinline__ bool clean_values(uint8_t* lds, int tid) {
+    constexpr uint32_t LIMIT = FMT == BF16 ? 0x7F80u : 0x7C00u;
+    bool found = false;
+#pragma unroll 1
+    for (int i = tid; i < 64 * D / 8; i += 256) {
+        const uint4 x = *reinterpret_cast<const uint4*>(lds + i * 16);
+        if (max_magnitude8(x) < LIMIT) continue;
+        auto clean = [](uint32_t w) {
+            return ((w & 0x7FFFu) >= LIMIT ? 0u : w & 0xFFFFu) | ((w >> 16 & 0x7FFFu) >= LIMIT ? 0u : w & 0xFFFF0000u);
+        };
+        *reinterpret_cast<uint4*>(lds + i * 16) = make_uint4(clean(x.x), clean(x.y), clean(x.z), clean(x.w));
+        found = true;
+    }
+    return found;
+}
+
 }  // namespace eco
