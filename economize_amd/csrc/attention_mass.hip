@@ -23,10 +23,9 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
     __shared__ __align__(16) float stat[2][64];
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
-    const int pairs = p.rows.sequences * p.kv_heads;
-    const int id = blockIdx.x;
-    if (id >= pairs * p.tiles) {  // the last workgroups: keys of no sequence
-        const int workers = gridDim.x - pairs * p.tiles, me = id - pairs * p.tiles;
+    const int work = gridDim.x - p.fill;
+    if (static_cast<int>(blockIdx.x) >= work) {  // the last workgroups: keys of no sequence
+        const int workers = p.fill, me = blockIdx.x - work;
         for (int g = 0; g <= p.rows.sequences; ++g) {
             int64_t from = g == 0 ? 0 : p.rows.k_end[g - 1];
             int64_t to = g == p.rows.sequences ? p.rows.k_rows : p.rows.k_begin[g];
@@ -37,7 +36,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
         }
         return;
     }
-    const int pair = id % pairs, first = id / pairs;
+    int pair, first;
+    if (!work_of(p.order, blockIdx.x, pair, first)) return;
     const int s = pair / p.kv_heads, kvh = pair % p.kv_heads;
     const Sequence seq = sequence_of(p.rows, s);
     const int tiles = (seq.nk + KEYS - 1) / KEYS;
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
     const int window_begin = p.window > 0 && p.window < seq.nq ? seq.nq - p.window : 0;
     const float c2 = p.scale * kLog2e, cc = CAP ? 1.0f : c2;
 
-    for (int t = first; t < tiles; t += p.tiles) {  // the first keys are seen by most queries: the longest work first
+    for (int t = first; t < tiles; t += p.order.tiles) {  // the first keys are seen by most queries: the longest work first
         const int wg0 = t * KEYS;
         const int key0 = wg0 + wave * 32 * KT;
         uint4 kf[KT][KS];
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
         TileLoad<D, THREADS> qt;
         float st = 0.0f;
         auto load = [&](int step) {
-            const int g = step / per_head, i0 = begin + 64 * (step % per_head);
+            const int g = step % p.groups, i0 = begin + 64 * (per_head - 1 - step / p.groups);
             const int head = kvh * p.groups + g;
             qt.load(p.q + seq.q0 * p.sq_t + head * p.sq_h, p.sq_t, i0, seq.nq, tid);
             if (tid < 64)
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
                 put(buf ^ 1);
                 if (step + 2 < steps) load(step + 2);
             }
-            const int i0 = begin + 64 * (step % per_head);
+            const int i0 = begin + 64 * (per_head - 1 - step / p.groups);
             if (key0 <= i0 + 63 + offset && key0 < seq.nk) {
                 const bool masked = key0 + 32 * KT - 1 > i0 + offset || i0 + 63 >= seq.nq;
 #pragma unroll
@@ -144,14 +144,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
 }
 
 template <int D, int FMT, int KT>
-int launch(MassParams p, int max_keys, hipStream_t stream) {
+int launch(MassParams p, int max_queries, int max_keys, hipStream_t stream) {
     constexpr int KEYS = WAVES * 32 * KT;
-    const int64_t pairs = static_cast<int64_t>(p.rows.sequences) * p.kv_heads;
-    int64_t tiles = (static_cast<int64_t>(max_keys) + KEYS - 1) / KEYS;
-    if (tiles * pairs > (1 << 28)) tiles = (1 << 28) / pairs;
-    if (tiles < 1) tiles = 1;
-    p.tiles = static_cast<int>(tiles);
-    const dim3 grid(static_cast<uint32_t>(tiles * pairs + (p.fill ? 8 : 0)));
+    p.order = work_order(static_cast<int64_t>(p.rows.sequences) * p.kv_heads, (static_cast<int64_t>(max_keys) + KEYS - 1) / KEYS,
+                         static_cast<int64_t>(max_queries) * p.groups * D * 2);
+    p.fill = p.fill ? 8 : 0;
+    const dim3 grid(static_cast<uint32_t>(p.order.blocks() + p.fill));
     if (p.softcap > 0.0f)
         hipLaunchKernelGGL((attention_mass_kernel<D, FMT, KT, true>), grid, dim3(THREADS), 0, stream, p);
     else
@@ -160,16 +158,16 @@ int launch(MassParams p, int max_keys, hipStream_t stream) {
 }
 
 template <int FMT>
-int launch_dim(const MassParams& p, int max_keys, hipStream_t stream) {
-    if (p.head_dim == 64) return launch<64, FMT, 2>(p, max_keys, stream);
-    if (p.head_dim == 128) return launch<128, FMT, 2>(p, max_keys, stream);
-    return launch<256, FMT, 1>(p, max_keys, stream);
+int launch_dim(const MassParams& p, int max_queries, int max_keys, hipStream_t stream) {
+    if (p.head_dim == 64) return launch<64, FMT, 2>(p, max_queries, max_keys, stream);
+    if (p.head_dim == 128) return launch<128, FMT, 2>(p, max_queries, max_keys, stream);
+    return launch<256, FMT, 1>(p, max_queries, max_keys, stream);
 }
 
 }  // namespace
 
-int attention_mass(const MassParams& p, int format, int max_keys, hipStream_t stream) {
-    return format == BF16 ? launch_dim<BF16>(p, max_keys, stream) : launch_dim<FP16>(p, max_keys, stream);
+int attention_mass(const MassParams& p, int format, int max_queries, int max_keys, hipStream_t stream) {
+    return format == BF16 ? launch_dim<BF16>(p, max_queries, max_keys, stream) : launch_dim<FP16>(p, max_queries, max_keys, stream);
 }
 
 }  // namespace eco

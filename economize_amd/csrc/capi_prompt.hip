@@ -97,6 +97,7 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
     if (lse && sl_h < q_rows) return fail("prompt attention: lse rows are shorter than the queries");
     if (max_queries < 0 || max_keys < 0) return fail("prompt attention: sizes must not be negative");
     if (static_cast<int64_t>(sequences) * kv_heads > (1 << 24)) return fail("prompt attention: too many sequences");
+    if (q_rows > 0x7fff0000 / (q_heads / kv_heads)) return fail("prompt attention: too many queries for one call");
     PromptParams p{};
     p.q = static_cast<const uint16_t*>(q);
     p.k = static_cast<const uint16_t*>(k);
@@ -143,7 +144,9 @@ int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h
     p.q_heads = q_heads, p.kv_heads = kv_heads, p.groups = q_heads / kv_heads, p.head_dim = head_dim;
     p.scale = scale, p.softcap = softcap;
     const int mk = static_cast<int>(max_keys < k_rows ? max_keys : k_rows);
-    return attention_mass(p, format, mk, static_cast<hipStream_t>(stream));
+    const int mq = static_cast<int>(max_queries < q_rows ? max_queries : q_rows);
+    const int counted = window > 0 && window < mq ? window : mq;
+    return attention_mass(p, format, counted, mk, static_cast<hipStream_t>(stream));
 }
 
 int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,

@@ -15,6 +15,29 @@ struct PackedRows {
     int64_t q_rows, k_rows;
 };
 
+// Which (sequence, KV head) pair and which of its tiles a workgroup takes. The tiles of a pair read the same rows, so they
+// run close together: the pairs in `group` at a time, their longest tiles first. Workgroups go to the eight XCDs in turn,
+// each with an L2 of its own: with `pin` a pair stays on one.
+struct WorkOrder {
+    int pairs, tiles, group, pin;
+    int per_xcd() const { return (pairs + 7) / 8; }
+    int64_t blocks() const { return static_cast<int64_t>(tiles) * (pin ? 8 * per_xcd() : pairs); }
+};
+
+// `tiles` per pair, whose rows read by all of them take `bytes`: as many pairs at a time as three quarters of an L2 hold.
+// Pinned where every XCD gets about as many pairs.
+inline WorkOrder work_order(int64_t pairs, int64_t tiles, int64_t bytes) {
+    if (tiles * pairs > (1 << 28)) tiles = (1 << 28) / pairs;
+    WorkOrder o;
+    o.pairs = static_cast<int>(pairs);
+    o.tiles = static_cast<int>(tiles < 1 ? 1 : tiles);
+    o.pin = pairs % 8 == 0 || pairs >= 64;
+    const int64_t fit = (3 << 20) / (bytes < 1 ? 1 : bytes);
+    const int64_t most = o.pin ? o.per_xcd() : pairs;
+    o.group = static_cast<int>(fit < 1 ? 1 : fit > most ? most : fit);
+    return o;
+}
+
 struct PromptParams {
     const uint16_t *q, *k, *v;
     int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h;  // element strides of tokens and heads
@@ -24,9 +47,10 @@ struct PromptParams {
     int64_t so_t, so_h;
     float* lse;  // [Hq, sl_h] or null
     int64_t sl_h;
-    int fill;                          // rows of no sequence: out 0 and lse -inf (1), or left as they are (0)
+    int fill;  // workgroups that give rows of no sequence out 0 and lse -inf (0: they are left as they are)
     int q_heads, kv_heads, groups, head_dim;
-    int tiles;      // row tiles a launch holds per sequence and KV head (longer sequences loop over them)
+    uint32_t group_inverse;
+    WorkOrder order;  // (sequences of more row tiles than the launch holds loop over them)
     float scale, softcap;
 };
 
@@ -43,13 +67,13 @@ struct MassParams {
     int64_t sl_h;
     float* mass;  // [Hkv, sm_h]
     int64_t sm_h;
-    int fill;    // keys of no sequence: 0 (1), or left as they are (0)
+    int fill;    // workgroups that give keys of no sequence 0 (0: they are left as they are)
     int window;  // only the last `window` queries of a sequence count
     int q_heads, kv_heads, groups, head_dim;
-    int tiles;  // key tiles a launch holds per sequence and KV head (longer sequences loop over them)
+    WorkOrder order;  // (sequences of more key tiles than the launch holds loop over them)
     float scale, softcap;
 };
 
-int attention_mass(const MassParams& p, int format, int max_keys, hipStream_t stream);
+int attention_mass(const MassParams& p, int format, int max_queries, int max_keys, hipStream_t stream);
 
 }  // namespace eco

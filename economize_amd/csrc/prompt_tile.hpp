@@ -61,6 +61,17 @@ __device__ __forceinline__ Sequence sequence_of(const PackedRows& r, int s) {
     return q;
 }
 
+// The pair and the tile (0 the longest) of workgroup id; false where there is none.
+__device__ __forceinline__ bool work_of(const WorkOrder& o, int id, int& pair, int& tile) {
+    const int lanes = o.pin ? 8 : 1, total = o.pin ? (o.pairs + 7) / 8 : o.pairs;
+    const int k = id / lanes, whole = o.tiles * o.group;
+    const int first = k / whole * o.group, within = k % whole;
+    const int width = total - first < o.group ? total - first : o.group;
+    tile = within / width;
+    pair = (first + within % width) * lanes + id % lanes;
+    return pair < o.pairs;
+}
+
 // A tile of 64 rows of D 16-bit channels in LDS, in chunks of 16 bytes. Keys are read as MFMA operands of 32 rows by 16
 // channels (ds_read_b128, lane l row l % 32), values transposed (ds_read_b64_tr_b16, 4 rows by 64 bytes for 32 lanes); the
 // two swizzles spread the rows of one such read over all 64 banks.
@@ -154,12 +165,12 @@ __device__ __forceinline__ uint2 lds_read_transposed(uint32_t at) {
 }
 
 // Copies of 64-row tiles straight into LDS (buffer_load_dwordx4 ... lds: 64 lanes' 16 bytes in a row from the address in
-// M0), by 256 threads. A lane's place in LDS is fixed, so it fetches the chunk the swizzle puts there. Rows past the
+// M0), by a workgroup of THREADS. A lane's place in LDS is fixed, so it fetches the chunk the swizzle puts there. Rows past the
 // sequence's end are outside the buffer resource. The copies of a tile complete at the workgroup's next tile_barrier.
-template <int D>
+template <int D, int THREADS>
 struct TileCopy {
-    static constexpr int CHUNKS = D / 8, N = 64 * CHUNKS / 256, ROWS = 256 / CHUNKS;  // rows per instruction of 4 waves
-    static constexpr int KINDS = D == 256 ? 2 : 1;  // the swizzle repeats every 16 rows
+    static constexpr int CHUNKS = D / 8, N = 64 * CHUNKS / THREADS, ROWS = THREADS / CHUNKS;  // rows per instruction
+    static constexpr int KINDS = ROWS < 16 ? 16 / ROWS : 1;  // the swizzle repeats every 16 rows
     uint32_t from[KINDS];
     int wave;
 
@@ -187,7 +198,7 @@ struct TileCopy {
         const uint32_t to = lds_address(lds) + wave * 1024u;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + i * 4096u);
+            const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + i * (THREADS * 16u));
             const uint32_t skip = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(i * ROWS) * static_cast<uint32_t>(stride * 2));
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                          :: "s"(m0), "v"(from[i % KINDS]), "s"(rsrc), "s"(skip) : "memory");
@@ -195,13 +206,13 @@ struct TileCopy {
     }
 };
 
-// Infinities and NaN of a tile of values in LDS to 0, by 256 threads; whether this thread found one.
-template <int D, int FMT>
+// Infinities and NaN of a tile of values in LDS to 0, by THREADS; whether this thread found one.
+template <int D, int FMT, int THREADS>
 __device__ __forceinline__ bool clean_values(uint8_t* lds, int tid) {
     constexpr uint32_t LIMIT = FMT == BF16 ? 0x7F80u : 0x7C00u;
     bool found = false;
 #pragma unroll 1
-    for (int i = tid; i < 64 * D / 8; i += 256) {
+    for (int i = tid; i < 64 * D / 8; i += THREADS) {
         const uint4 x = *reinterpret_cast<const uint4*>(lds + i * 16);
         if (max_magnitude8(x) < LIMIT) continue;
         auto clean = [](uint32_t w) {
