@@ -99,8 +99,9 @@ SIGNATURES: dict[str, tuple[type | None, list]] = {
     "eco_prompt_attention_workspace_size": (c_size_t, [_I, _I, _I, _I, _I, _I]),
     "eco_prompt_attention": (c_int32, [_P, _I, _L, _L, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _I, _I,
                                        _P, _P, _L, _L, _P, _L, _I, _I, _I, _I, _F, _F, _P, _S, _P]),
+    "eco_attention_mass_workspace_size": (c_size_t, [_I, _L, _I, _I, _I]),
     "eco_attention_mass": (c_int32, [_P, _I, _L, _L, _P, _L, _L, _P, _L, _P, _P, _P, _P, _I, _L, _L, _I, _I, _I,
-                                     _P, _L, _I, _I, _I, _I, _F, _F, _P]),
+                                     _P, _L, _I, _I, _I, _I, _F, _F, _P, _S, _P]),
     "eco_evict_prompt": (c_int32, [_P, _P, _L, _L, _L, _L, _P, _L, _P, _P, _L, _I, _P, _P, _P, _P, _P, _P,
                                    _I, _I, _I, _I, _I, _I, _P]),
     "eco_heavy_hitter_workspace_size": (c_size_t, [_I, _I, _I, _I, _I]),

@@ -1,10 +1,12 @@
 // The attention weight every key of packed prompts receives: mass[h, j] = sum over the queries i that see key j (all, or
 // the last `window` of its sequence) and the query heads of KV head h of exp(x_ij - lse_i), from the softmax statistics
-// lse_i the attention left. No running maximum is needed and no query is read twice by a workgroup.
+// lse_i the attention left: one product, no running maximum.
 //
-// A wave holds 64 keys as columns in registers and streams the queries of the group's heads through LDS: S = Q K^T puts
-// one key in each lane with 16 of 32 queries in its registers, so a weight is added where it is computed, in fp32 and in
-// a fixed order: no atomics, the same bits every time.
+// A wave holds 32 KT keys as columns in registers and streams the queries of the group's heads through LDS, 64 at a time:
+// S = Q K^T puts one key in each lane with 16 of 32 queries in its registers, so a weight is added where it is computed, in
+// fp32 and in a fixed order: no atomics, the same bits every time. The products of 32 queries run while the weights of the
+// 32 before are computed. All tiles of a (sequence, KV head) walk the queries from the last down, so they read the same ones
+// at the same time. Long walks are cut by heads, each a workgroup of its own, summed by mass_sum_kernel.
 
 #include "prompt_tile.hpp"
 
@@ -17,12 +19,14 @@ constexpr int THREADS = WAVES * 64;
 
 template <int D, int FMT, int KT, bool CAP>
 __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p) {
+    typedef Tile<D> T;
     constexpr int KS = D / 16;
     constexpr int KEYS = WAVES * 32 * KT;
-    __shared__ __align__(16) uint8_t lds[2][Tile<D>::BYTES];
-    __shared__ __align__(16) float stat[2][64];
+    __shared__ __align__(256) uint8_t lds[2][T::BYTES];
+    __shared__ __align__(16) float stat[4][64];
 
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int col = lane & 31, half = lane >> 5;
     const int work = gridDim.x - p.fill;
     if (static_cast<int>(blockIdx.x) >= work) {  // the last workgroups: keys of no sequence
         const int workers = p.fill, me = blockIdx.x - work;
@@ -36,18 +40,25 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
         }
         return;
     }
-    int pair, first;
-    if (!work_of(p.order, blockIdx.x, pair, first)) return;
+    int pair, slot;
+    if (!work_of(p.order, blockIdx.x, pair, slot)) return;
+    const int part = slot % p.parts, first = slot / p.parts, stride = p.order.tiles / p.parts;
     const int s = pair / p.kv_heads, kvh = pair % p.kv_heads;
     const Sequence seq = sequence_of(p.rows, s);
     const int tiles = (seq.nk + KEYS - 1) / KEYS;
     const int offset = seq.nk - seq.nq;
     const int window_begin = p.window > 0 && p.window < seq.nq ? seq.nq - p.window : 0;
-    const float c2 = p.scale * kLog2e, cc = CAP ? 1.0f : c2;
+    const int heads = p.groups / p.parts;
+    const float cc = CAP ? 1.0f : p.scale * kLog2e;
+    const TileCopy<D, THREADS> copy(tid, p.sq_t, true);
+    const uint32_t place = col * (D * 2) + T::key_chunk(col, half) * 16;
 
-    for (int t = first; t < tiles; t += p.order.tiles) {  // the first keys are seen by most queries: the longest work first
-        const int wg0 = t * KEYS;
-        const int key0 = wg0 + wave * 32 * KT;
+    for (int t = first; t < tiles; t += stride) {  // the first keys are seen by most queries: the longest work first
+        int begin = t * KEYS - offset;  // the first query that counts and sees one of the tile's keys
+        if (begin < window_begin) begin = window_begin;
+        const int per_head = begin < seq.nq ? (seq.nq - begin + 63) / 64 : 0;
+        const int steps = per_head * heads;  // of 64 queries, from the last down to `begin`, heads innermost
+        const int key0 = t * KEYS + wave * 32 * KT;
         uint4 kf[KT][KS];
         float sum[KT];
 #pragma unroll
@@ -58,103 +69,160 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
             for (int i = 0; i < KS; ++i) kf[u][i] = *reinterpret_cast<const uint4*>(kp + 16 * i);
             sum[u] = 0.0f;
         }
-        int begin = wg0 - offset;
-        if (begin < window_begin) begin = window_begin;
-        const int per_head = begin < seq.nq ? (seq.nq - begin + 63) / 64 : 0;
-        const int steps = per_head * p.groups;
-        TileLoad<D, THREADS> qt;
-        float st = 0.0f;
-        auto load = [&](int step) {
-            const int g = step % p.groups, i0 = begin + 64 * (per_head - 1 - step / p.groups);
-            const int head = kvh * p.groups + g;
-            qt.load(p.q + seq.q0 * p.sq_t + head * p.sq_h, p.sq_t, i0, seq.nq, tid);
-            if (tid < 64)
-                st = i0 + tid < seq.nq ? p.lse[head * p.sl_h + seq.q0 + i0 + tid] * kLog2e : INFINITY;
-        };
-        auto put = [&](int buf) {
-            qt.template store<true>(lds[buf], tid);
-            if (tid < 64) stat[buf][tid] = st;
-        };
-        if (steps > 0) load(0);
-        __syncthreads();
-        if (steps > 0) put(0);
-        if (steps > 1) load(1);
-        __syncthreads();
-        for (int step = 0; step < steps; ++step) {
-            const int buf = step & 1;
-            if (step + 1 < steps) {
-                put(buf ^ 1);
-                if (step + 2 < steps) load(step + 2);
+        float st = 0.0f;  // the next step's statistics, on their way (the first wave's)
+        // The step under way (its first query) and the one fetched next (its first query and head).
+        int now = 0, next = begin + 64 * (per_head - 1), next_head = 0;
+        const uint16_t* qbase = p.q + seq.q0 * p.sq_t + (kvh * p.groups + part * heads) * p.sq_h;
+        const float* lbase = p.lse + (kvh * p.groups + part * heads) * p.sl_h + seq.q0;
+        auto fetch = [&](int step) {
+            copy.start(lds[step & 1], qbase + next_head * p.sq_h, p.sq_t, next, seq.nq);
+            if (wave == 0) {
+                const int i = next + lane < seq.nq ? next + lane : seq.nq - 1;
+                st = lbase[next_head * p.sl_h + i];
             }
-            const int i0 = begin + 64 * (per_head - 1 - step / p.groups);
-            if (key0 <= i0 + 63 + offset && key0 < seq.nk) {
-                const bool masked = key0 + 32 * KT - 1 > i0 + offset || i0 + 63 >= seq.nq;
+        };
+        auto arrive = [&](int step) {  // step's queries and statistics are there
+            if (wave == 0) stat[step & 3][lane] = st * kLog2e;
+            tile_barrier();
+            now = next;
+            if (++next_head == heads) {
+                next_head = 0;
+                next -= 64;
+            }
+            if (step + 1 < steps) fetch(step + 1);
+        };
+        auto scores = [&](int step, int b, f32x16 (&x)[KT]) {
+            uint32_t at = lds_address(lds[step & 1]) + place + b * 32 * (D * 2);
+            asm volatile("" : "+v"(at));
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    f32x16 x[KT];
+            for (int u = 0; u < KT; ++u) x[u] = f32x16{};
 #pragma unroll
-                    for (int u = 0; u < KT; ++u) x[u] = f32x16{};
-                    const int row = 32 * b + col;
+            for (int i = 0; i < KS; ++i) {
+                const uint4 qf = lds_read16(at ^ (32 * i));
 #pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-                        const uint4 qf = *reinterpret_cast<const uint4*>(
-                            lds[buf] + row * (D * 2) + Tile<D>::key_chunk(row, 2 * i + half) * 16);
+                for (int u = 0; u < KT; ++u) x[u] = mfma32<FMT>(qf, kf[u][i], x[u]);
+            }
+        };
+        auto hide = [&](int b, f32x16 (&x)[KT]) {  // soft cap, and the queries that do not see the lane's key
+            if constexpr (CAP) {
 #pragma unroll
-                        for (int u = 0; u < KT; ++u) x[u] = mfma32<FMT>(qf, kf[u][i], x[u]);
-                    }
-                    float4 ls[4];
+                for (int u = 0; u < KT; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        ls[i] = *reinterpret_cast<const float4*>(&stat[buf][32 * b + 8 * i + 4 * half]);
+                    for (int i = 0; i < 16; ++i) x[u][i] = soft_cap_log2(x[u][i] * p.scale, p.softcap, 1.0f / p.softcap);
+            }
+            const int i0 = now + 32 * b;
+            if (key0 + 32 * KT - 1 > i0 + offset || i0 + 31 >= seq.nq) {
 #pragma unroll
-                    for (int u = 0; u < KT; ++u) {
+                for (int u = 0; u < KT; ++u) {
+                    const int lo = key0 + 32 * u + col - offset - i0 - 4 * half, hi = seq.nq - i0 - 4 * half;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const float4 four = ls[r >> 2];
-                            const float l = (r & 3) == 0 ? four.x : (r & 3) == 1 ? four.y : (r & 3) == 2 ? four.z : four.w;
-                            float y = x[u][r];
-                            if constexpr (CAP) y = soft_cap_log2(y * p.scale, p.softcap, 1.0f / p.softcap);
-                            x[u][r] = __builtin_fmaf(y, cc, -l);
-                        }
-                        if (masked) {
-                            asm volatile("" ::: );  // (a branch of its own: as selects the masks would cost every tile)
-                            const int key = key0 + 32 * u + col;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) {
-                                const int i = i0 + 32 * b + 8 * (r >> 2) + 4 * half + (r & 3);
-                                if (key > i + offset || i >= seq.nq) x[u][r] = -INFINITY;
-                            }
-                        }
-                        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // short sums first: their rounding stays small
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) part[r & 3] += __builtin_amdgcn_exp2f(x[u][r]);
-                        sum[u] += (part[0] + part[1]) + (part[2] + part[3]);
+                    for (int i = 0; i < 16; ++i) {
+                        const int e = 8 * (i >> 2) + (i & 3);
+                        if (e < lo || e >= hi) x[u][i] = -INFINITY;
                     }
                 }
             }
-            __syncthreads();
+        };
+        auto weights = [&](int step, int b, const f32x16 (&x)[KT]) {
+            float4 ls[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                ls[i] = *reinterpret_cast<const float4*>(&stat[step & 3][32 * b + 8 * i + 4 * half]);
+#pragma unroll
+            for (int u = 0; u < KT; ++u) {
+                float part4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // short sums first: their rounding stays small
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float4 f = ls[i >> 2];
+                    const float l = (i & 3) == 0 ? f.x : (i & 3) == 1 ? f.y : (i & 3) == 2 ? f.z : f.w;
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], cc, -l));
+                    part4[i & 3] = i < 4 ? y : part4[i & 3] + y;
+                }
+                sum[u] += (part4[0] + part4[1]) + (part4[2] + part4[3]);
+            }
+        };
+        // The products of half b of a step into nxt, under the weights of the half before, in cur.
+        auto both = [&](int step, int b, f32x16 (&nxt)[KT], const f32x16 (&cur)[KT]) {
+            scores(step, b, nxt);
+            weights(b ? step : step - 1, b ^ 1, cur);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, KT, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, (52 * KT + KS - 1) / KS, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < KT; ++u) asm volatile("" : "+v"(sum[u]));  // (the weights belong before the masks)
+            hide(b, nxt);
+        };
+        f32x16 xa[KT], xb[KT];
+        tile_barrier();  // the previous tile's reads are done
+        if (steps > 0) {
+            fetch(0);
+            arrive(0);
+            scores(0, 0, xa);
+            hide(0, xa);
+            int step = 0;
+            for (; step + 1 < steps; ++step) {
+                both(step, 1, xb, xa);
+                arrive(step + 1);
+                both(step + 1, 0, xa, xb);
+            }
+            both(step, 1, xb, xa);
+            weights(step, 1, xb);
         }
+        float* to = p.parts == 1 ? p.mass + kvh * p.sm_h
+                                 : p.partial + (static_cast<int64_t>(part) * p.kv_heads + kvh) * p.rows.k_rows;
 #pragma unroll
         for (int u = 0; u < KT; ++u) {
-            const float total = swap_sum(sum[u]);
+            const float all = swap_sum(sum[u]);
             const int key = key0 + 32 * u + col;
-            if (half == 0 && key < seq.nk) p.mass[kvh * p.sm_h + seq.k0 + key] = total;
+            if (half == 0 && key < seq.nk) to[seq.k0 + key] = all;
         }
     }
+}
+
+// The parts, in order.
+__global__ __launch_bounds__(256) void mass_sum_kernel(MassParams p) {
+    const int s = blockIdx.y / p.kv_heads, kvh = blockIdx.y % p.kv_heads;
+    const Sequence seq = sequence_of(p.rows, s);
+    for (int key = blockIdx.x * 256 + threadIdx.x; key < seq.nk; key += gridDim.x * 256) {
+        float sum = 0.0f;
+        for (int c = 0; c < p.parts; ++c)
+            sum += p.partial[(static_cast<int64_t>(c) * p.kv_heads + kvh) * p.rows.k_rows + seq.k0 + key];
+        p.mass[kvh * p.sm_h + seq.k0 + key] = sum;
+    }
+}
+
+constexpr int keys_per_tile(int head_dim) { return WAVES * 32 * (head_dim == 256 ? 1 : 2); }
+
+// Walks of 64 steps and more are cut by heads: their lengths differ up to the whole, and shorter ones even out.
+int parts_of(int max_queries, int groups) {
+    return (static_cast<int64_t>(max_queries) + 63) / 64 * groups >= 64 ? groups : 1;
 }
 
 template <int D, int FMT, int KT>
 int launch(MassParams p, int max_queries, int max_keys, hipStream_t stream) {
     constexpr int KEYS = WAVES * 32 * KT;
-    p.order = work_order(static_cast<int64_t>(p.rows.sequences) * p.kv_heads, (static_cast<int64_t>(max_keys) + KEYS - 1) / KEYS,
-                         static_cast<int64_t>(max_queries) * p.groups * D * 2);
-    p.fill = p.fill ? 8 : 0;
-    const dim3 grid(static_cast<uint32_t>(p.order.blocks() + p.fill));
+    static_assert(KEYS == keys_per_tile(D), "one tile size per head dim");
+    const int64_t pairs = static_cast<int64_t>(p.rows.sequences) * p.kv_heads;
+    const int64_t tiles = (static_cast<int64_t>(max_keys) + KEYS - 1) / KEYS;
+    const int64_t bytes = static_cast<int64_t>(max_queries) * p.groups * D * 2;
+    p.order = work_order(pairs, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
+    p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
+    const int fill = p.fill ? 8 : 0;
+    p.fill = fill;
+    const dim3 grid(static_cast<uint32_t>(p.order.blocks() + fill));
     if (p.softcap > 0.0f)
         hipLaunchKernelGGL((attention_mass_kernel<D, FMT, KT, true>), grid, dim3(THREADS), 0, stream, p);
     else
         hipLaunchKernelGGL((attention_mass_kernel<D, FMT, KT, false>), grid, dim3(THREADS), 0, stream, p);
-    return check_launch("attention_mass_kernel");
+    if (int rc = check_launch("attention_mass_kernel")) return rc;
+    if (p.parts == 1) return 0;
+    const int64_t blocks = (static_cast<int64_t>(max_keys) + 255) / 256;
+    hipLaunchKernelGGL(mass_sum_kernel, dim3(static_cast<uint32_t>(blocks < 1 ? 1 : blocks), static_cast<uint32_t>(pairs)),
+                       dim3(256), 0, stream, p);
+    return check_launch("mass_sum_kernel");
 }
 
 template <int FMT>
@@ -166,8 +234,19 @@ int launch_dim(const MassParams& p, int max_queries, int max_keys, hipStream_t s
 
 }  // namespace
 
-int attention_mass(const MassParams& p, int format, int max_queries, int max_keys, hipStream_t stream) {
-    return format == BF16 ? launch_dim<BF16>(p, max_queries, max_keys, stream) : launch_dim<FP16>(p, max_queries, max_keys, stream);
+size_t attention_mass_workspace(int max_queries, int64_t k_rows, int q_heads, int kv_heads) {
+    const int parts = parts_of(max_queries, q_heads / kv_heads);
+    return parts == 1 ? 0 : static_cast<size_t>(parts) * kv_heads * k_rows * sizeof(float);
+}
+
+int attention_mass(MassParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
+                   hipStream_t stream) {
+    p.parts = parts_of(max_queries, p.groups);
+    const size_t need = attention_mass_workspace(max_queries, p.rows.k_rows, p.q_heads, p.kv_heads);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return fail("attention mass: the workspace is too small");
+    p.partial = static_cast<float*>(workspace);
+    return format == BF16 ? launch_dim<BF16>(p, max_queries, max_keys, stream)
+                          : launch_dim<FP16>(p, max_queries, max_keys, stream);
 }
 
 }  // namespace eco

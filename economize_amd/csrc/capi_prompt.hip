@@ -96,7 +96,7 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
     if (int rc = check_rows("prompt attention: outputs", out, {so_t, so_h})) return rc;
     if (lse && sl_h < q_rows) return fail("prompt attention: lse rows are shorter than the queries");
     if (max_queries < 0 || max_keys < 0) return fail("prompt attention: sizes must not be negative");
-    if (static_cast<int64_t>(sequences) * kv_heads > (1 << 24)) return fail("prompt attention: too many sequences");
+    if (static_cast<int64_t>(sequences) * kv_heads > 65535) return fail("prompt attention: too many sequences");
     if (q_rows > 0x7fff0000 / (q_heads / kv_heads)) return fail("prompt attention: too many queries for one call");
     PromptParams p{};
     p.q = static_cast<const uint16_t*>(q);
@@ -116,11 +116,18 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
     return prompt_attention(p, format, mq, mk, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
+size_t eco_attention_mass_workspace_size(int32_t max_queries, int64_t k_rows, int32_t window, int32_t q_heads,
+                                         int32_t kv_heads) {
+    if (max_queries < 0 || k_rows < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads) return 0;
+    return attention_mass_workspace(window > 0 && window < max_queries ? window : max_queries, k_rows, q_heads, kv_heads);
+}
+
 int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t,
                        int64_t sk_h, const float* lse, int64_t sl_h, const int32_t* q_begin, const int32_t* q_end,
                        const int32_t* k_begin, const int32_t* k_end, int32_t sequences, int64_t q_rows, int64_t k_rows,
                        int32_t max_queries, int32_t max_keys, int32_t window, float* mass, int64_t sm_h, int32_t fill,
-                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap, void* stream) {
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap, void* workspace,
+                       size_t workspace_bytes, void* stream) {
     const char* what = "attention mass";
     if (k_rows == 0) return 0;
     if (!k || !mass || (q_rows > 0 && (!q || !lse))) return fail("attention mass: null pointer");
@@ -131,8 +138,9 @@ int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h
     if (int rc = check_rows("attention mass: keys", k, {sk_t, sk_h})) return rc;
     if (sl_h < q_rows) return fail("attention mass: lse rows are shorter than the queries");
     if (sm_h < k_rows) return fail("attention mass: mass rows are shorter than the keys");
+    if (q_rows > 0x7fff0000 / (q_heads / kv_heads)) return fail("attention mass: too many queries for one call");
     if (window < 0 || max_queries < 0 || max_keys < 0) return fail("attention mass: sizes must not be negative");
-    if (static_cast<int64_t>(sequences) * kv_heads > (1 << 24)) return fail("attention mass: too many sequences");
+    if (static_cast<int64_t>(sequences) * kv_heads > 65535) return fail("attention mass: too many sequences");
     MassParams p{};
     p.q = static_cast<const uint16_t*>(q);
     p.k = static_cast<const uint16_t*>(k);
@@ -143,10 +151,8 @@ int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h
     p.fill = fill, p.window = window;
     p.q_heads = q_heads, p.kv_heads = kv_heads, p.groups = q_heads / kv_heads, p.head_dim = head_dim;
     p.scale = scale, p.softcap = softcap;
-    const int mk = static_cast<int>(max_keys < k_rows ? max_keys : k_rows);
-    const int mq = static_cast<int>(max_queries < q_rows ? max_queries : q_rows);
-    const int counted = window > 0 && window < mq ? window : mq;
-    return attention_mass(p, format, counted, mk, static_cast<hipStream_t>(stream));
+    const int counted = window > 0 && window < max_queries ? window : max_queries;
+    return attention_mass(p, format, counted, max_keys, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,

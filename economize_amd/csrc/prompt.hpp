@@ -71,9 +71,13 @@ struct MassParams {
     int window;  // only the last `window` queries of a sequence count
     int q_heads, kv_heads, groups, head_dim;
     WorkOrder order;  // (sequences of more key tiles than the launch holds loop over them)
+    int parts;       // a key tile's query heads are cut into so many parts (1, or one per head)
+    float* partial;  // [parts, Hkv, k_rows] where parts > 1
     float scale, softcap;
 };
 
-int attention_mass(const MassParams& p, int format, int max_queries, int max_keys, hipStream_t stream);
+int attention_mass(MassParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
+                   hipStream_t stream);
+size_t attention_mass_workspace(int max_queries, int64_t k_rows, int q_heads, int kv_heads);
 
 }  // namespace eco

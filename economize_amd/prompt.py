@@ -179,11 +179,15 @@ def attention_mass(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu
     max_k = keys if max_seqlen_k is None else min(int(max_seqlen_k), keys)
     if cu_seqlens_k is None and max_seqlen_k is None:
         max_k = max_q
+    window = min(int(window or 0), 0x7fffffff)
     with _lib.on(device):
+        need = _lib.lib().eco_attention_mass_workspace_size(max_q, keys, window, q_heads, kv_heads)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         _lib.call(
             "eco_attention_mass", query.data_ptr(), _lib.fmt(query.dtype), *strides_of(query), key.data_ptr(),
             *strides_of(key), lse.data_ptr(), lse.stride(0) if q_heads > 1 else tokens, q_begin, q_end, k_begin, k_end,
-            sequences, tokens, keys, max_q, max_k, min(int(window or 0), 0x7fffffff), out.data_ptr(),
+            sequences, tokens, keys, max_q, max_k, window, out.data_ptr(),
             out.stride(0) if kv_heads > 1 else keys, int(fill), q_heads, kv_heads, head_dim,
-            float(1 / math.sqrt(head_dim) if scale is None else scale), float(softcap or 0.0), _lib.stream_of(device))
+            float(1 / math.sqrt(head_dim) if scale is None else scale), float(softcap or 0.0), _lib.ptr(ws), need,
+            _lib.stream_of(device))
     return out

@@ -487,12 +487,16 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
 
 /* The attention weight every key received: mass[h, j] (fp32 [Hkv, sm_h]) = the sum over the queries that see key j (with
  * window > 0 the last `window` of its sequence) and the query heads of KV head h of exp(score - lse). Keys of no
- * sequence: 0 with fill, else left as they are. */
+ * sequence: 0 with fill, else left as they are. The workspace (sized for the same max_queries) holds the sums of long
+ * walks' parts. At most 65535 sequences times KV heads. */
+size_t eco_attention_mass_workspace_size(int32_t max_queries, int64_t k_rows, int32_t window, int32_t q_heads,
+                                         int32_t kv_heads);
 int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t,
                        int64_t sk_h, const float* lse, int64_t sl_h, const int32_t* q_begin, const int32_t* q_end,
                        const int32_t* k_begin, const int32_t* k_end, int32_t sequences, int64_t q_rows, int64_t k_rows,
                        int32_t max_queries, int32_t max_keys, int32_t window, float* mass, int64_t sm_h, int32_t fill,
-                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap, void* stream);
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* A cache held at a budget of `slots` per row and KV head: keys / values [B, Hkv, slots, D], score fp32 and position
  * int32 [B, Hkv, slots], count int32 [B, Hkv] filled slots, length int32 [B] tokens seen, all contiguous. The first

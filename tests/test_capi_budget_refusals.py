@@ -26,7 +26,8 @@ BASE = {
         null=("sinks", "workspace", "stream"), **ROWS, **SHAPE, sq_t=512, sq_h=64, sk_t=128, sk_h=64, sv_t=128, sv_h=64,
         so_t=512, so_h=64, sl_h=30, fill=1, workspace_bytes=1 << 40),
     "eco_attention_mass": dict(
-        null=("stream",), **ROWS, **SHAPE, sq_t=512, sq_h=64, sk_t=128, sk_h=64, sl_h=30, window=0, sm_h=30, fill=1),
+        null=("workspace", "stream"), **ROWS, **SHAPE, sq_t=512, sq_h=64, sk_t=128, sk_h=64, sl_h=30, window=0, sm_h=30,
+        fill=1, workspace_bytes=0),
     "eco_evict_prompt": dict(
         null=("stream",), **CACHE, sk_t=128, sk_h=64, sv_t=128, sv_h=64, sm_h=30, rows=30, max_tokens=20),
     "eco_heavy_hitter_decode": dict(
@@ -51,6 +52,7 @@ CASES = [
     ("eco_prompt_attention", dict(sl_h=29), "lse rows are shorter"),
     ("eco_prompt_attention", dict(max_queries=-1), "must not be negative"),
     ("eco_attention_mass", dict(lse=None), "null pointer"),
+    ("eco_attention_mass", dict(max_queries=30000, max_keys=30000), "workspace is too small"),
     ("eco_attention_mass", dict(window=-1), "must not be negative"),
     ("eco_attention_mass", dict(sm_h=29), "mass rows are shorter"),
     ("eco_attention_mass", dict(k=FAKE + 2), "keys must be 16-byte aligned"),
