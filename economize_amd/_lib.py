@@ -96,7 +96,7 @@ SIGNATURES: dict[str, tuple[type | None, list]] = {
                                          _P, _P, _I, _I, _I,  # counts, bits, groups
                                          _P, _L, _L, _L, _L, _P, _P, _L, _L, _L,  # mask, sinks, out
                                          _I, _I, _I, _I, _I, _I, _I, _F, _F, _P, _S, _P]),
-    "eco_prompt_attention_workspace_size": (c_size_t, [_I, _I, _I, _I, _I, _I]),
+    "eco_prompt_attention_workspace_size": (c_size_t, [_I, _L, _I, _I, _I, _I, _I]),
     "eco_prompt_attention": (c_int32, [_P, _I, _L, _L, _P, _P, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _I, _I,
                                        _P, _P, _L, _L, _P, _L, _I, _I, _I, _I, _F, _F, _P, _S, _P]),
     "eco_attention_mass_workspace_size": (c_size_t, [_I, _L, _I, _I, _I]),

@@ -70,11 +70,12 @@ using namespace eco;
 
 extern "C" {
 
-size_t eco_prompt_attention_workspace_size(int32_t sequences, int32_t max_queries, int32_t max_keys, int32_t q_heads,
-                                           int32_t kv_heads, int32_t head_dim) {
-    if (sequences <= 0 || max_queries < 0 || max_keys < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads)
+size_t eco_prompt_attention_workspace_size(int32_t sequences, int64_t q_rows, int32_t max_queries, int32_t max_keys,
+                                           int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
+    if (sequences <= 0 || q_rows < 0 || max_queries < 0 || max_keys < 0 || q_heads <= 0 || kv_heads <= 0 ||
+        q_heads % kv_heads)
         return 0;
-    return prompt_attention_workspace(sequences, max_queries, max_keys, q_heads, kv_heads, head_dim);
+    return prompt_attention_workspace(sequences, q_rows, max_queries, max_keys, q_heads, kv_heads, head_dim);
 }
 
 int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, const void* v,
@@ -111,9 +112,8 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
     p.fill = fill;
     p.q_heads = q_heads, p.kv_heads = kv_heads, p.groups = q_heads / kv_heads, p.head_dim = head_dim;
     p.scale = scale, p.softcap = softcap;
-    const int mq = static_cast<int>(max_queries < q_rows ? max_queries : q_rows);
-    const int mk = static_cast<int>(max_keys < k_rows ? max_keys : k_rows);
-    return prompt_attention(p, format, mq, mk, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+    if (!aligned16(workspace)) return fail("prompt attention: the workspace must be 16-byte aligned");
+    return prompt_attention(p, format, max_queries, max_keys, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 size_t eco_attention_mass_workspace_size(int32_t max_queries, int64_t k_rows, int32_t window, int32_t q_heads,

@@ -34,7 +34,9 @@ inline WorkOrder work_order(int64_t pairs, int64_t tiles, int64_t bytes) {
     o.pin = pairs % 8 == 0 || pairs >= 64;
     const int64_t fit = (3 << 20) / (bytes < 1 ? 1 : bytes);
     const int64_t most = o.pin ? o.per_xcd() : pairs;
-    o.group = static_cast<int>(fit < 1 ? 1 : fit > most ? most : fit);
+    // (an odd number: workgroups in turn go to the four shader engines of an XCD, and where only every other pair has
+    // tiles left, two of the engines would be idle)
+    o.group = static_cast<int>(fit < 1 ? 1 : fit > most ? most : fit - (fit % 2 == 0));
     return o;
 }
 
@@ -51,12 +53,14 @@ struct PromptParams {
     int q_heads, kv_heads, groups, head_dim;
     uint32_t group_inverse;
     WorkOrder order;  // (sequences of more row tiles than the launch holds loop over them)
+    int parts;                     // a row tile's keys are cut into up to so many
+    float *part_out, *part_stats;  // [parts, q_rows, Hq, D] and [.., 2], of the row tiles that were cut
     float scale, softcap;
 };
 
-int prompt_attention(const PromptParams& p, int format, int max_queries, int max_keys, void* workspace,
-                     size_t workspace_bytes, hipStream_t stream);
-size_t prompt_attention_workspace(int sequences, int max_queries, int max_keys, int q_heads, int kv_heads,
+int prompt_attention(PromptParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
+                     hipStream_t stream);
+size_t prompt_attention_workspace(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads,
                                   int head_dim);
 
 struct MassParams {

@@ -18,6 +18,18 @@ namespace {
 
 constexpr float NEVER = -1e30f;  // running maximum before the first key (log2 units)
 
+constexpr int MIN_PART = 8;  // tiles of 64 keys a part holds at least: its rows' sums are written and read once more
+
+// The parts of a row tile that sees so many tiles of keys, and the first tile of a part.
+__device__ __forceinline__ int parts_of(const PromptParams& p, int key_tiles) {
+    const int n = key_tiles / MIN_PART;
+    return n < 1 ? 1 : n < p.parts ? n : p.parts;
+}
+
+__device__ __forceinline__ int part_begin(int key_tiles, int part, int parts) {
+    return static_cast<int>(static_cast<int64_t>(key_tiles) * part / parts);
+}
+
 template <int D, int FMT, int QT, int WAVES, bool CAP>
 __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) void prompt_attention_kernel(PromptParams p) {
     constexpr int THREADS = WAVES * 64;
@@ -50,8 +62,10 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
         }
         return;
     }
-    int pair, first;
-    if (!work_of(p.order, blockIdx.x, pair, first)) return;
+    int pair, slot;
+    if (!work_of(p.order, blockIdx.x, pair, slot)) return;
+    // (parts outermost: workgroups without work come last, where they leave no shader engine without any)
+    const int stride = p.order.tiles / p.parts, part = slot / stride, first = slot % stride;
     const int s = pair / p.kv_heads, kvh = pair % p.kv_heads;
     const Sequence seq = sequence_of(p.rows, s);
     const int total = seq.nq * p.groups;  // (below 2^31: the host checks)
@@ -73,22 +87,26 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
     const uint32_t kplace = col * (D * 2) + T::key_chunk(col, half) * 16;
     const uint32_t vplace = vrow * (D * 2) + T::value_chunk(vrow, ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
 
-    for (int t = first; t < tiles; t += p.order.tiles) {
+    for (int t = first; t < tiles; t += stride) {
         const int low_row = (tiles - 1 - t) * ROWS;  // the longest rows first
         const int row0 = low_row + wave * 32 * QT;
         const int last = over_groups(low_row + ROWS - 1 < total ? low_row + ROWS - 1 : total - 1) + offset;
         const int full = over_groups(low_row) + offset;  // every row of the tile sees keys <= full, some keys <= last
         const int wave_full = over_groups(row0 < total ? row0 : total - 1) + offset;
-        const int key_tiles = last < 0 ? 0 : (last >> 6) + 1;
+        // The part's tiles of keys: from `from` up to key_tiles, of the row tile's all_tiles
+        const int all_tiles = last < 0 ? 0 : (last >> 6) + 1;
+        const int parts = parts_of(p, all_tiles);
+        if (part >= parts) continue;
+        const int from = part_begin(all_tiles, part, parts), key_tiles = part_begin(all_tiles, part + 1, parts);
 
         auto keys = [&](int j) { kcopy.start(lds[j & 1], kbase, p.sk_t, 64 * j, seq.nk); };
         auto values = [&](int j) { vcopy.start(lds[2 + (j & 1)], vbase, p.sv_t, 64 * j, seq.nk); };
         if (t != first) tile_barrier();  // the previous row tile's reads are done
         if (tid == 0) unseen = 0;
-        if (key_tiles > 0) {
-            keys(0);
-            values(0);
-            if (key_tiles > 1) keys(1);
+        if (key_tiles > from) {
+            keys(from);
+            values(from);
+            if (key_tiles > from + 1) keys(from + 1);
         }
         int qi[QT], head[QT], limit[QT];
         uint4 qf[QT][KS];
@@ -250,13 +268,13 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
             raise(nxt);
         };
 
-        if (key_tiles > 0) {
+        if (key_tiles > from) {
             tile_barrier();
-            scores(0, sa);
-            hide(0, sa);
+            scores(from, sa);
+            hide(from, sa);
             raise(sa);
         }
-        int j = 0;
+        int j = from;
         for (; j + 2 < key_tiles; j += 2) {
             step(j, sa, sb);
             step(j + 1, sb, sa);
@@ -277,7 +295,8 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
         }
         __syncthreads();
         if (unseen) {
-            for (int key = (full + 1) & ~63; key <= last; ++key) {
+            const int unseen_from = (full + 1) & ~63, upto = last < 64 * key_tiles - 1 ? last : 64 * key_tiles - 1;
+            for (int key = unseen_from > 64 * from ? unseen_from : 64 * from; key <= upto; ++key) {
                 const uint16_t* vp = vbase + key * p.sv_t + 4 * half;
 #pragma unroll
                 for (int u = 0; u < QT; ++u)
@@ -301,6 +320,20 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
             const float sum = swap_sum(l0[u] + l1[u]);
             const int h = kvh * p.groups + head[u];
             const int64_t token = seq.q0 + qi[u];
+            if (parts > 1) {  // the part's maximum, sum and products, joined with the others by prompt_join_kernel
+                if (row0 + 32 * u + col < total) {
+                    const int64_t row = (static_cast<int64_t>(part) * p.rows.q_rows + token) * p.q_heads + h;
+                    if (half == 0) *reinterpret_cast<float2*>(p.part_stats + 2 * row) = make_float2(m[u], sum);
+                    float* to = p.part_out + row * D + 4 * half;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<float4*>(to + 32 * d + 8 * i) =
+                                make_float4(acc[u][d][4 * i], acc[u][d][4 * i + 1], acc[u][d][4 * i + 2], acc[u][d][4 * i + 3]);
+                }
+                continue;
+            }
             float scale = 1.0f, den = sum, top = m[u];
             if (p.sinks) {
                 const float sink = p.sinks[h] * kLog2e;
@@ -333,12 +366,74 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
     }
 }
 
+// The parts of the rows whose keys were cut: half a wave to a row and 32 channels.
+template <int D, int FMT, int ROWS>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
+    int pair, first;
+    if (!work_of(p.order, blockIdx.x, pair, first)) return;
+    const int kvh = pair % p.kv_heads;
+    const Sequence seq = sequence_of(p.rows, pair / p.kv_heads);
+    const int total = seq.nq * p.groups, tiles = (total + ROWS - 1) / ROWS, offset = seq.nk - seq.nq;
+    constexpr int LANES = D / 4;  // to a row
+    const int sub = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    for (int t = first; t < tiles; t += p.order.tiles) {
+        const int top = (t + 1) * ROWS - 1 < total ? (t + 1) * ROWS - 1 : total - 1;
+        const int last = top / p.groups + offset, all_tiles = last < 0 ? 0 : (last >> 6) + 1;
+        const int parts = parts_of(p, all_tiles);
+        if (parts == 1) continue;
+        for (int r = t * ROWS + sub; r <= top; r += 256 / LANES) {
+            const int qi = r / p.groups, h = kvh * p.groups + r - qi * p.groups;
+            const int64_t token = seq.q0 + qi, row = token * p.q_heads + h, step = p.rows.q_rows * p.q_heads;
+            float most = NEVER;
+            if (p.sinks) most = p.sinks[h] * kLog2e > most ? p.sinks[h] * kLog2e : most;
+            for (int c = 0; c < parts; ++c) {
+                const float m = p.part_stats[2 * (row + c * step)];
+                most = m > most ? m : most;
+            }
+            float den = p.sinks ? __builtin_amdgcn_exp2f(p.sinks[h] * kLog2e - most) : 0.0f;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int c = 0; c < parts; ++c) {
+                const float2 st = *reinterpret_cast<const float2*>(p.part_stats + 2 * (row + c * step));
+                const float4 x = *reinterpret_cast<const float4*>(p.part_out + (row + c * step) * D + 4 * lane);
+                const float w = __builtin_amdgcn_exp2f(st.x - most);
+                den += st.y * w;
+                y.x += x.x * w;
+                y.y += x.y * w;
+                y.z += x.z * w;
+                y.w += x.w * w;
+            }
+            const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+            *reinterpret_cast<uint2*>(p.out + token * p.so_t + h * p.so_h + 4 * lane) =
+                make_uint2(pack_pair<FMT>(y.x * inv, y.y * inv), pack_pair<FMT>(y.z * inv, y.w * inv));
+            if (p.lse && lane == 0) p.lse[h * p.sl_h + token] = (most + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
+        }
+    }
+}
+
+// Where there are too few row tiles for the GPU (four to a CU), their keys are cut into up to so many parts.
+int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads) {
+    constexpr int ROWS = 128;
+    const int64_t groups = q_heads / kv_heads;
+    const int64_t by_longest = (max_queries * groups + ROWS - 1) / ROWS * sequences;
+    const int64_t by_rows = q_rows * groups / ROWS + sequences;
+    const int64_t row_tiles = (by_longest < by_rows ? by_longest : by_rows) * kv_heads;
+    const int64_t most = static_cast<int64_t>(max_keys) / (64 * MIN_PART);
+    const int64_t parts = row_tiles > 0 ? (1024 + row_tiles - 1) / row_tiles : 1;
+    return static_cast<int>(parts < 1 || most < 1 ? 1 : parts < most ? parts : most);
+}
+
+size_t part_bytes(int parts, int64_t q_rows, int q_heads, int floats) {
+    return parts == 1 ? 0 : static_cast<size_t>(parts) * q_rows * q_heads * floats * sizeof(float);
+}
+
 template <int D, int FMT, int QT, int WAVES>
 int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
     constexpr int ROWS = WAVES * 32 * QT;
-    const int64_t rows = static_cast<int64_t>(max_queries) * p.groups;
-    p.order = work_order(static_cast<int64_t>(p.rows.sequences) * p.kv_heads, (rows + ROWS - 1) / ROWS,
-                         static_cast<int64_t>(max_keys) * D * 4);
+    const int64_t pairs = static_cast<int64_t>(p.rows.sequences) * p.kv_heads;
+    const int64_t tiles = (static_cast<int64_t>(max_queries) * p.groups + ROWS - 1) / ROWS;
+    const int64_t bytes = static_cast<int64_t>(max_keys) * D * 4;
+    p.order = work_order(pairs, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
+    p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
     p.group_inverse = static_cast<uint32_t>((0x100000000ull + p.groups - 1) / p.groups);
     p.fill = p.fill ? 32 : 0;
     const dim3 grid(static_cast<uint32_t>(p.order.blocks() + p.fill));
@@ -346,7 +441,12 @@ int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
         hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, QT, WAVES, true>), grid, dim3(WAVES * 64), 0, stream, p);
     else
         hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, QT, WAVES, false>), grid, dim3(WAVES * 64), 0, stream, p);
-    return check_launch("prompt_attention_kernel");
+    if (int rc = check_launch("prompt_attention_kernel")) return rc;
+    if (p.parts == 1) return 0;
+    p.order = work_order(pairs, tiles, bytes);
+    hipLaunchKernelGGL((prompt_join_kernel<D, FMT, ROWS>), dim3(static_cast<uint32_t>(p.order.blocks())), dim3(256), 0,
+                       stream, p);
+    return check_launch("prompt_join_kernel");
 }
 
 template <int FMT>
@@ -358,11 +458,21 @@ int launch_dim(const PromptParams& p, int max_queries, int max_keys, hipStream_t
 
 }  // namespace
 
-size_t prompt_attention_workspace(int, int, int, int, int, int) { return 0; }
+size_t prompt_attention_workspace(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads,
+                                  int head_dim) {
+    return part_bytes(most_parts(sequences, q_rows, max_queries, max_keys, q_heads, kv_heads), q_rows, q_heads, head_dim + 2);
+}
 
-int prompt_attention(const PromptParams& p, int format, int max_queries, int max_keys, void*, size_t,
+int prompt_attention(PromptParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
                      hipStream_t stream) {
-    return format == BF16 ? launch_dim<BF16>(p, max_queries, max_keys, stream) : launch_dim<FP16>(p, max_queries, max_keys, stream);
+    p.parts = most_parts(p.rows.sequences, p.rows.q_rows, max_queries, max_keys, p.q_heads, p.kv_heads);
+    if (p.parts > 1 && (!workspace || workspace_bytes < part_bytes(p.parts, p.rows.q_rows, p.q_heads, p.head_dim + 2)))
+        return fail("prompt attention: the workspace is too small");
+    p.part_out = static_cast<float*>(workspace);
+    p.part_stats = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                            part_bytes(p.parts, p.rows.q_rows, p.q_heads, p.head_dim));
+    return format == BF16 ? launch_dim<BF16>(p, max_queries, max_keys, stream)
+                          : launch_dim<FP16>(p, max_queries, max_keys, stream);
 }
 
 }  // namespace eco

@@ -127,7 +127,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if cu_seqlens_k is None and max_seqlen_k is None:
         max_k = max_q
     with _lib.on(device):
-        need = int(_lib.lib().eco_prompt_attention_workspace_size(sequences, max_q, max_k, q_heads, key.shape[1], head_dim))
+        need = _lib.lib().eco_prompt_attention_workspace_size(sequences, tokens, max_q, max_k, q_heads, key.shape[1],
+                                                              head_dim)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         _lib.call(
             "eco_prompt_attention", query.data_ptr(), _lib.fmt(query.dtype), *strides_of(query), key.data_ptr(),

@@ -473,10 +473,11 @@ int eco_kivi_packed_decode(const void* q, int32_t q_format, int64_t sq_b, int64_
 
 /* Causal attention of every sequence's queries over its own keys: out [q_rows, Hq, D] and lse [Hq, sl_h] (optional, fp32:
  * the logarithm of the softmax denominator, sinks [Hq] included). A query that sees no key gives 0 and lse -inf (its
- * sink's logit with sinks). Rows of no sequence: 0 and -inf with fill, else left as they are. The workspace (optional
- * where its size is 0) holds the parts of rows whose keys are cut. */
-size_t eco_prompt_attention_workspace_size(int32_t sequences, int32_t max_queries, int32_t max_keys, int32_t q_heads,
-                                           int32_t kv_heads, int32_t head_dim);
+ * sink's logit with sinks). Rows of no sequence: 0 and -inf with fill, else left as they are. The workspace (sized
+ * for the same bounds; NULL where its size is 0) holds the parts of rows whose keys are cut. At most 65535 sequences times
+ * KV heads. */
+size_t eco_prompt_attention_workspace_size(int32_t sequences, int64_t q_rows, int32_t max_queries, int32_t max_keys,
+                                           int32_t q_heads, int32_t kv_heads, int32_t head_dim);
 int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, const void* v,
                          int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h, const int32_t* q_begin,
                          const int32_t* q_end, const int32_t* k_begin, const int32_t* k_end, int32_t sequences,

@@ -51,6 +51,9 @@ CASES = [
     ("eco_prompt_attention", dict(out=FAKE + 8), "outputs must be 16-byte aligned"),
     ("eco_prompt_attention", dict(sl_h=29), "lse rows are shorter"),
     ("eco_prompt_attention", dict(max_queries=-1), "must not be negative"),
+    ("eco_prompt_attention", dict(max_keys=30000, workspace_bytes=0), "workspace is too small"),
+    ("eco_prompt_attention", dict(sequences=40000), "too many sequences"),
+    ("eco_prompt_attention", dict(q_rows=1 << 30, sl_h=1 << 30), "too many queries"),
     ("eco_attention_mass", dict(lse=None), "null pointer"),
     ("eco_attention_mass", dict(max_queries=30000, max_keys=30000), "workspace is too small"),
     ("eco_attention_mass", dict(window=-1), "must not be negative"),
@@ -118,7 +121,7 @@ def test_workspaces() -> None:
     lib = _lib.lib()
     assert lib.eco_heavy_hitter_workspace_size(2, 8, 2, 64, 64) > 0
     assert lib.eco_heavy_hitter_workspace_size(2, 7, 2, 64, 64) == 0
-    assert lib.eco_prompt_attention_workspace_size(2, 10, 10, 7, 2, 64) == 0
+    assert lib.eco_prompt_attention_workspace_size(2, 20, 10, 10, 7, 2, 64) == 0
 
 
 def test_caches_and_rows_are_checked() -> None:

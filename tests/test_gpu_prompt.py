@@ -93,6 +93,33 @@ def test_softcap_sinks_scale_window(dtype, dim) -> None:
     check(q, k, v, cu, cu, lens, lens, scale=0.5, sinks=sinks, softcap=50.0, window=1000)
 
 
+@pytest.mark.parametrize("lens_q,lens_k", [([1], [9000]), ([3, 130, 0, 1], [2000, 5000, 0, 64]), ([40, 7], [4095, 513]),
+                                           ([600], [1700])])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (FP16, 64), (BF16, 256)])
+def test_few_queries_behind_many_keys(lens_q, lens_k, dtype, dim) -> None:
+    """Too few rows for the GPU: their keys are cut into parts and joined."""
+    from economize_amd import _lib
+
+    heads = (6, 2)
+    q, k, v, cu_q, cu_k = prompt_inputs(17, lens_q, lens_k, heads, dim, dtype)
+    assert _lib.lib().eco_prompt_attention_workspace_size(len(lens_q), sum(lens_q), max(lens_q), max(lens_k), *heads,
+                                                          dim) > 0
+    sinks = torch.randn(6, generator=torch.Generator().manual_seed(2)).cuda()
+    check(q, k, v, cu_q, cu_k, lens_q, lens_k)
+    check(q, k, v, cu_q, cu_k, lens_q, lens_k, sinks=sinks, softcap=30.0, window=2)
+    out = torch.full((sum(lens_q) + 5, 6, dim), 2.0, dtype=dtype, device="cuda")
+    run(torch.cat([q, q[:1].expand(5, -1, -1)]), k, v, cu_q, cu_k, lens_q, lens_k, out=out)
+    assert (out[-5:] == 2).all()
+
+
+def test_unseen_nan_in_a_cut_row() -> None:
+    """The keys are cut, and the last tiles hold infinities that only the last queries see."""
+    q, k, v, cu_q, cu_k = prompt_inputs(18, [100], [3000], (4, 2), 128, BF16)
+    v[2999, 0, 5], v[2950, 1, 9], v[2890, 0, 77] = math.inf, math.nan, -math.inf
+    out, _, _ = check(q, k, v, cu_q, cu_k, [100], [3000])
+    assert torch.isfinite(out[:99, :2, 5]).all() and torch.isinf(out[99, :2, 5]).all()
+
+
 def test_sinks_without_keys() -> None:
     """A query without keys attends to its sink alone: 0, and the sink's logit as its denominator's logarithm."""
     q, k, v, cu_q, cu_k = prompt_inputs(2, [70], [5], (4, 2), 64, BF16)
@@ -195,9 +222,10 @@ def test_bounds_of_the_launch_do_not_bound_the_result() -> None:
     lens = [900, 1, 300]
     q, k, v, cu, _ = prompt_inputs(12, lens, lens, (4, 1), 128, BF16)
     want, lse = prompt_attention(q, k, v, cu, 900, return_lse=True)
-    for bound in (0, 1, 100, None):
-        got = prompt_attention(q, k, v, cu, bound)
-        assert torch.equal(got, want), bound
+    rows = cu.cpu().numpy()
+    exact, _, size = ob.prompt_attention(f64(q), f64(k), f64(v), rows, rows, 128 ** -0.5)
+    for bound in (0, 1, 100, 900, None):  # (the bound decides how long rows are cut, so the bits may differ)
+        assert_output(prompt_attention(q, k, v, cu, bound), exact, size, score_error(q, k, 128 ** -0.5, 900))
     # (the bound decides how a long walk is cut: the same positive terms, summed in another order, each sum within
     # (terms / 32 + 32) 2^-24 of its value)
     mass = attention_mass(q, k, lse, cu, 900)
@@ -205,7 +233,7 @@ def test_bounds_of_the_launch_do_not_bound_the_result() -> None:
     for bound in (0, 1, 300, None):
         torch.testing.assert_close(attention_mass(q, k, lse, cu, bound), mass, rtol=rtol, atol=0)
     wild = torch.tensor([-5, 900, 901, 99999], dtype=torch.int32, device="cuda")
-    assert torch.equal(prompt_attention(q, k, v, wild), want)
+    assert torch.equal(prompt_attention(q, k, v, wild, 900), want)
 
 
 def test_no_rows() -> None:
