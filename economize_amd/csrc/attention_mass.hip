@@ -208,7 +208,7 @@ int launch(MassParams p, int max_queries, int max_keys, hipStream_t stream) {
     const int64_t pairs = static_cast<int64_t>(p.rows.sequences) * p.kv_heads;
     const int64_t tiles = (static_cast<int64_t>(max_keys) + KEYS - 1) / KEYS;
     const int64_t bytes = static_cast<int64_t>(max_queries) * p.groups * D * 2;
-    p.order = work_order(pairs, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
+    p.order = work_order(p.rows.sequences, p.kv_heads, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
     p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
     const int fill = p.fill ? 8 : 0;
     p.fill = fill;

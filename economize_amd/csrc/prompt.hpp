@@ -25,13 +25,15 @@ struct WorkOrder {
 };
 
 // `tiles` per pair, whose rows read by all of them take `bytes`: as many pairs at a time as three quarters of an L2 hold.
-// Pinned where every XCD gets about as many pairs.
-inline WorkOrder work_order(int64_t pairs, int64_t tiles, int64_t bytes) {
+// Pinned where that leaves the XCDs about the same work: with KV heads in eights each gets every sequence, otherwise many
+// sequences even out (6 sequences of different lengths with 4 KV heads, pinned: half of the CUs' time idle).
+inline WorkOrder work_order(int sequences, int kv_heads, int64_t tiles, int64_t bytes) {
+    const int64_t pairs = static_cast<int64_t>(sequences) * kv_heads;
     if (tiles * pairs > (1 << 28)) tiles = (1 << 28) / pairs;
     WorkOrder o;
     o.pairs = static_cast<int>(pairs);
     o.tiles = static_cast<int>(tiles < 1 ? 1 : tiles);
-    o.pin = pairs % 8 == 0 || pairs >= 64;
+    o.pin = kv_heads % 8 == 0 || pairs >= 128;
     const int64_t fit = (3 << 20) / (bytes < 1 ? 1 : bytes);
     const int64_t most = o.pin ? o.per_xcd() : pairs;
     // (an odd number: workgroups in turn go to the four shader engines of an XCD, and where only every other pair has

@@ -366,7 +366,9 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
     }
 }
 
-// The parts of the rows whose keys were cut: half a wave to a row and 32 channels.
+// The parts of the rows whose keys were cut: four channels to a lane, JOINED rows of a row tile to a workgroup.
+constexpr int JOINED = 32;
+
 template <int D, int FMT, int ROWS>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
     int pair, first;
@@ -381,26 +383,45 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
         const int last = top / p.groups + offset, all_tiles = last < 0 ? 0 : (last >> 6) + 1;
         const int parts = parts_of(p, all_tiles);
         if (parts == 1) continue;
-        for (int r = t * ROWS + sub; r <= top; r += 256 / LANES) {
+        for (int r = t * ROWS + blockIdx.y * JOINED + sub; r <= top && r < t * ROWS + (blockIdx.y + 1) * JOINED;
+             r += 256 / LANES) {
             const int qi = r / p.groups, h = kvh * p.groups + r - qi * p.groups;
             const int64_t token = seq.q0 + qi, row = token * p.q_heads + h, step = p.rows.q_rows * p.q_heads;
-            float most = NEVER;
-            if (p.sinks) most = p.sinks[h] * kLog2e > most ? p.sinks[h] * kLog2e : most;
-            for (int c = 0; c < parts; ++c) {
-                const float m = p.part_stats[2 * (row + c * step)];
-                most = m > most ? m : most;
+            float most = NEVER, den = 0.0f;
+            if (p.sinks && p.sinks[h] * kLog2e > NEVER) {
+                most = p.sinks[h] * kLog2e;
+                den = 1.0f;
             }
-            float den = p.sinks ? __builtin_amdgcn_exp2f(p.sinks[h] * kLog2e - most) : 0.0f;
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int c = 0; c < parts; ++c) {
-                const float2 st = *reinterpret_cast<const float2*>(p.part_stats + 2 * (row + c * step));
-                const float4 x = *reinterpret_cast<const float4*>(p.part_out + (row + c * step) * D + 4 * lane);
-                const float w = __builtin_amdgcn_exp2f(st.x - most);
-                den += st.y * w;
-                y.x += x.x * w;
-                y.y += x.y * w;
-                y.z += x.z * w;
-                y.w += x.w * w;
+            for (int c0 = 0; c0 < parts; c0 += 4) {  // four parts' loads in flight
+                float2 st[4];
+                float4 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t at = row + (c0 + i < parts ? c0 + i : parts - 1) * step;
+                    st[i] = *reinterpret_cast<const float2*>(p.part_stats + 2 * at);
+                    x[i] = *reinterpret_cast<const float4*>(p.part_out + at * D + 4 * lane);
+                }
+                float top4 = most;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top4 = st[i].x > top4 ? st[i].x : top4;
+                const float a = __builtin_amdgcn_exp2f(most - top4);
+                most = top4;
+                den *= a;
+                y.x *= a;
+                y.y *= a;
+                y.z *= a;
+                y.w *= a;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (c0 + i >= parts) continue;
+                    const float w = __builtin_amdgcn_exp2f(st[i].x - most);
+                    den += st[i].y * w;
+                    y.x += x[i].x * w;
+                    y.y += x[i].y * w;
+                    y.z += x[i].z * w;
+                    y.w += x[i].w * w;
+                }
             }
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;
             *reinterpret_cast<uint2*>(p.out + token * p.so_t + h * p.so_h + 4 * lane) =
@@ -410,7 +431,8 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
     }
 }
 
-// Where there are too few row tiles for the GPU (four to a CU), their keys are cut into up to so many parts.
+// Where there are too few row tiles for the GPU (six to a CU: prompt chunks of 6 sequences take 147 us at four, 142 at six,
+// 164 at sixteen), their keys are cut into up to so many parts.
 int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads) {
     constexpr int ROWS = 128;
     const int64_t groups = q_heads / kv_heads;
@@ -418,7 +440,7 @@ int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int
     const int64_t by_rows = q_rows * groups / ROWS + sequences;
     const int64_t row_tiles = (by_longest < by_rows ? by_longest : by_rows) * kv_heads;
     const int64_t most = static_cast<int64_t>(max_keys) / (64 * MIN_PART);
-    const int64_t parts = row_tiles > 0 ? (1024 + row_tiles - 1) / row_tiles : 1;
+    const int64_t parts = row_tiles > 0 ? (1536 + row_tiles - 1) / row_tiles : 1;
     return static_cast<int>(parts < 1 || most < 1 ? 1 : parts < most ? parts : most);
 }
 
@@ -429,10 +451,9 @@ size_t part_bytes(int parts, int64_t q_rows, int q_heads, int floats) {
 template <int D, int FMT, int QT, int WAVES>
 int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
     constexpr int ROWS = WAVES * 32 * QT;
-    const int64_t pairs = static_cast<int64_t>(p.rows.sequences) * p.kv_heads;
     const int64_t tiles = (static_cast<int64_t>(max_queries) * p.groups + ROWS - 1) / ROWS;
     const int64_t bytes = static_cast<int64_t>(max_keys) * D * 4;
-    p.order = work_order(pairs, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
+    p.order = work_order(p.rows.sequences, p.kv_heads, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
     p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
     p.group_inverse = static_cast<uint32_t>((0x100000000ull + p.groups - 1) / p.groups);
     p.fill = p.fill ? 32 : 0;
@@ -443,9 +464,9 @@ int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
         hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, QT, WAVES, false>), grid, dim3(WAVES * 64), 0, stream, p);
     if (int rc = check_launch("prompt_attention_kernel")) return rc;
     if (p.parts == 1) return 0;
-    p.order = work_order(pairs, tiles, bytes);
-    hipLaunchKernelGGL((prompt_join_kernel<D, FMT, ROWS>), dim3(static_cast<uint32_t>(p.order.blocks())), dim3(256), 0,
-                       stream, p);
+    p.order = work_order(p.rows.sequences, p.kv_heads, tiles, bytes);
+    hipLaunchKernelGGL((prompt_join_kernel<D, FMT, ROWS>), dim3(static_cast<uint32_t>(p.order.blocks()), ROWS / JOINED),
+                       dim3(256), 0, stream, p);
     return check_launch("prompt_join_kernel");
 }
 
