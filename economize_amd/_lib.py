@@ -7,7 +7,6 @@ The library is loaded on first use and never replaced by anything else: if it is
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
@@ -110,7 +109,6 @@ SIGNATURES: dict[str, tuple[type | None, list]] = {
 }
 
 _lib: ctypes.CDLL | None = None
-_HERE = contextlib.nullcontext()
 
 
 def lib() -> ctypes.CDLL:
@@ -157,11 +155,13 @@ def stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-def on(device: torch.device) -> contextlib.AbstractContextManager:
-    """``device`` as the current one for a launch (nothing to do when it is already)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+def call_on(device: torch.device, name: str, *args) -> None:
+    """:func:`call` with ``device`` as the current one, on its current stream (the last argument, added here)."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return call(name, *args, stream_of(device))
+    with torch.cuda.device(device):
+        return call(name, *args, stream_of(device))
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

@@ -13,13 +13,6 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int current_cus() {
-    int device = 0, cus = 0;
-    if (hipGetDevice(&device) != hipSuccess) return 256;
-    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0) return 256;
-    return cus;
-}
-
 int check_shape(const char* what, int format, int q_heads, int kv_heads, int head_dim, float scale, float softcap) {
     const std::string w = what;
     if (format != BF16 && format != FP16) return fail(w + ": queries, keys and values must be bf16 or fp16");
@@ -182,7 +175,7 @@ int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, i
 size_t eco_heavy_hitter_workspace_size(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t slots,
                                        int32_t head_dim) {
     if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || slots <= 0 || q_heads % kv_heads) return 0;
-    return heavy_hitter_workspace(batch, q_heads, kv_heads, slots, head_dim, current_cus());
+    return heavy_hitter_workspace(batch, q_heads, kv_heads, slots, head_dim);
 }
 
 int eco_heavy_hitter_decode(const void* q, int32_t format, int64_t sq_b, int64_t sq_h, const void* k, const void* v,
@@ -214,7 +207,7 @@ int eco_heavy_hitter_decode(const void* q, int32_t format, int64_t sq_b, int64_t
     p.so_b = so_b, p.so_h = so_h;
     p.q_heads = q_heads, p.groups = q_heads / kv_heads;
     p.scale = scale, p.softcap = softcap;
-    return heavy_hitter_decode(p, format, workspace, workspace_bytes, current_cus(), static_cast<hipStream_t>(stream));
+    return heavy_hitter_decode(p, format, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

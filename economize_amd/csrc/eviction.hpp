@@ -41,14 +41,15 @@ struct HeavyParams {
     int q_heads, groups;
     int splits, span;  // parts a row's slots are cut into, slots of a part
     float scale, softcap;
-    float* logits;   // workspace: [B, Hkv, G, C]
-    float* partial;  // [B, Hkv, splits, G, D + 2]
+    int pitch;       // slots of a row of `logits`: C in whole fours
+    float* logits;   // workspace: [B, Hkv, G, pitch]
+    float* partial;  // [B, Hkv, splits, G, D]
+    float* stats;    // [B, Hkv, splits, G, 2]: maximum and sum
     int32_t* plan;   // [B, Hkv, 4]: the slot written, filled slots, position
 };
 
-size_t heavy_hitter_workspace(int batch, int q_heads, int kv_heads, int slots, int head_dim, int cus);
-int heavy_hitter_decode(HeavyParams p, int format, void* workspace, size_t workspace_bytes, int cus,
-                        hipStream_t stream);
+size_t heavy_hitter_workspace(int batch, int q_heads, int kv_heads, int slots, int head_dim);
+int heavy_hitter_decode(HeavyParams p, int format, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 // Order of scores as unsigned integers: a NaN below everything, -0 equal to 0.
 __device__ __forceinline__ uint32_t score_rank(float x) {

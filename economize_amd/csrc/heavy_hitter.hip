@@ -7,7 +7,8 @@
 // heads as columns (S^T = K Q^T, v_mfma_f32_16x16x32: one head per lane), so P^T is the second product's operand with
 // values read transposed from LDS. The scaled scores go to the workspace with the part's maximum, sum and outputs.
 // heavy_merge_kernel: the parts' join, and the weights from the scores kept, added to the slots' scores. Every sum has a
-// fixed order: no atomics.
+// fixed order: no atomics. (The join by the last part of a row to finish, in the same launch, took as long for 2048 slots of
+// 4 heads, 57.6 us against 55.0, and twice as long for one row of 8192, 83 against 44.)
 
 #include <cstdlib>
 #include "eviction.hpp"
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(THREADS, (D == 256 ? 1 : 2)) void heavy_attend_kern
         plan[2] = token;
     }
     const int s1 = end < n ? end : n;
-    float* logits = p.logits + (static_cast<int64_t>(bh) * p.groups + head) * c.slots;
+    float* logits = p.logits + (static_cast<int64_t>(bh) * p.groups + head) * p.pitch;
 
     f32x4 acc[DT];
 #pragma unroll
@@ -187,14 +188,16 @@ __global__ __launch_bounds__(THREADS, (D == 256 ? 1 : 2)) void heavy_attend_kern
             for (int r = 0; r < 4; ++r) {
                 const int slot = k0 + 16 * v + 4 * grp + r;
                 float y = p.softcap > 0.0f ? soft_cap_log2(x[v][r] * p.scale, p.softcap, 1.0f / p.softcap) : x[v][r] * c2;
-                if (slot < s1) {
-                    if (head_there) logits[slot] = y;
-                } else {
-                    y = -INFINITY;
-                }
+                if (slot >= s1) y = -INFINITY;
                 x[v][r] = y;
                 mx = max_nan(mx, y);
             }
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {  // (rows of the workspace are whole fours)
+            const int slot = k0 + 16 * v + 4 * grp;
+            if (!head_there || slot >= s1) continue;
+            *reinterpret_cast<float4*>(logits + slot) = make_float4(x[v][0], x[v][1], x[v][2], x[v][3]);
+        }
         mx = group_max(mx);
         const float mn = mx > m ? mx : m;
         const float a = __builtin_amdgcn_exp2f(m - mn);
@@ -262,100 +265,138 @@ __global__ __launch_bounds__(THREADS, (D == 256 ? 1 : 2)) void heavy_attend_kern
     }
     __syncthreads();
     const int heads = p.groups - block * 16 < 16 ? p.groups - block * 16 : 16;
-    float* part = p.partial + ((static_cast<int64_t>(bh) * p.splits + split) * p.groups + block * 16) * (D + 2);
+    const int64_t at = (static_cast<int64_t>(bh) * p.splits + split) * p.groups + block * 16;
     for (int i = tid; i < heads * D; i += THREADS) {
         const int g = i / D, d = i % D;
         float y = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) y += joined[(w * 16 + g) * JP + d];
-        part[g * (D + 2) + 2 + d] = y;
+        p.partial[(at + g) * D + d] = y;
     }
-    if (tid < heads) {
-        part[tid * (D + 2)] = top;
-        part[tid * (D + 2) + 1] = sum;
-    }
+    if (tid < heads) *reinterpret_cast<float2*>(p.stats + 2 * (at + tid)) = make_float2(top, sum);
 }
 
+// The maximum and the sum of a head over its parts' (and its sink), by one wave.
+__device__ __forceinline__ float2 head_stats(const HeavyParams& p, int bh, int g, int lane) {
+    const float2* st = reinterpret_cast<const float2*>(p.stats) + static_cast<int64_t>(bh) * p.splits * p.groups + g;
+    float top = NEVER, sum = 0.0f;
+    for (int s = lane; s < p.splits; s += 64) {
+        const float2 x = st[static_cast<int64_t>(s) * p.groups];
+        const float to = x.x > top ? x.x : top;
+        sum = sum * __builtin_amdgcn_exp2f(top - to) + x.y * __builtin_amdgcn_exp2f(x.x - to);
+        top = to;
+    }
+    float most = top;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const float o = __shfl_xor(most, d);
+        most = o > most ? o : most;
+    }
+    const float sink = p.sinks ? p.sinks[bh % p.cache.kv_heads * p.groups + g] * kLog2e : NEVER;
+    most = sink > most ? sink : most;
+    sum *= __builtin_amdgcn_exp2f(top - most);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    if (p.sinks) sum += __builtin_amdgcn_exp2f(sink - most);
+    return make_float2(most, sum);
+}
+
+// The parts' join: the first p.groups workgroups of a row and KV head give one head's output each, the others the scores of
+// 4 THREADS slots each.
 template <int D, int FMT>
 __global__ __launch_bounds__(THREADS) void heavy_merge_kernel(HeavyParams p) {
-    __shared__ float lse[64], weight[64];
     const BudgetCache& c = p.cache;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int bh = blockIdx.x, b = bh / c.kv_heads, h = bh % c.kv_heads;
     const int32_t* plan = p.plan + 4 * static_cast<int64_t>(bh);
     const int to = plan[0], n = plan[1], token = plan[2];
-    const int64_t step = static_cast<int64_t>(p.groups) * (D + 2);
-    const float* part = p.partial + static_cast<int64_t>(bh) * p.splits * step;
-    if (tid < p.groups) {
-        float top = NEVER;
-        for (int s = 0; s < p.splits; ++s) {
-            const float m = part[s * step + tid * (D + 2)];
-            top = m > top ? m : top;
+    if (static_cast<int>(blockIdx.y) < p.groups) {
+        constexpr int SHARES = THREADS / D;  // threads to a channel, each a share of the parts
+        __shared__ float shares[THREADS];
+        const int g = blockIdx.y, d = tid % D, share = tid / D;
+        const float2 st = head_stats(p, bh, g, lane);
+        const float2* stats = reinterpret_cast<const float2*>(p.stats) + static_cast<int64_t>(bh) * p.splits * p.groups + g;
+        const float* x = p.partial + (static_cast<int64_t>(bh) * p.splits * p.groups + g) * D + d;
+        float y = 0.0f;
+        for (int s0 = share; s0 < p.splits; s0 += 8 * SHARES) {  // eight parts' loads in flight
+            float m[8], v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int s = s0 + i * SHARES < p.splits ? s0 + i * SHARES : s0;
+                m[i] = stats[static_cast<int64_t>(s) * p.groups].x;
+                v[i] = x[static_cast<int64_t>(s) * p.groups * D];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (s0 + i * SHARES < p.splits) y += v[i] * __builtin_amdgcn_exp2f(m[i] - st.x);
         }
-        if (p.sinks) {
-            const float sink = p.sinks[h * p.groups + tid] * kLog2e;
-            top = sink > top ? sink : top;
+        if constexpr (SHARES > 1) {
+            shares[tid] = y;
+            __syncthreads();
+            if (share > 0) return;
+            y = 0.0f;
+#pragma unroll
+            for (int i = 0; i < SHARES; ++i) y += shares[i * D + d];
         }
-        float sum = 0.0f;
-        for (int s = 0; s < p.splits; ++s)
-            sum += part[s * step + tid * (D + 2) + 1] * __builtin_amdgcn_exp2f(part[s * step + tid * (D + 2)] - top);
-        if (p.sinks) sum += __builtin_amdgcn_exp2f(p.sinks[h * p.groups + tid] * kLog2e - top);
-        lse[tid] = top + __builtin_amdgcn_logf(sum);
-        weight[tid] = 1.0f / sum;
-        // (the parts' weights are taken relative to `top` again below)
+        p.out[b * p.so_b + (h * p.groups + g) * p.so_h + d] =
+            static_cast<uint16_t>(pair16<FMT>(y / st.y, 0.0f) & 0xFFFFu);
+        return;
+    }
+    __shared__ float lse[64];
+    for (int g = wave; g < p.groups; g += WAVES) {
+        const float2 st = head_stats(p, bh, g, lane);
+        if (lane == 0) lse[g] = st.x + __builtin_amdgcn_logf(st.y);
     }
     __syncthreads();
-    if (blockIdx.y == 0) {
-        for (int i = tid; i < p.groups * D; i += THREADS) {
-            const int g = i / D, d = i % D;
-            float top = NEVER, y = 0.0f;
-            for (int s = 0; s < p.splits; ++s) {
-                const float m = part[s * step + g * (D + 2)];
-                top = m > top ? m : top;
-            }
-            if (p.sinks) {
-                const float sink = p.sinks[h * p.groups + g] * kLog2e;
-                top = sink > top ? sink : top;
-            }
-            for (int s = 0; s < p.splits; ++s)
-                y += part[s * step + g * (D + 2) + 2 + d] * __builtin_amdgcn_exp2f(part[s * step + g * (D + 2)] - top);
-            p.out[b * p.so_b + (h * p.groups + g) * p.so_h + d] =
-                static_cast<uint16_t>(pair16<FMT>(y * weight[g], 0.0f) & 0xFFFFu);
-        }
-        if (tid == 0) {
-            c.position[static_cast<int64_t>(bh) * c.slots + to] = token;
-            c.count[bh] = n;
-            if (h == 0) c.length[b] = token + 1;
-        }
+    const int s0 = (blockIdx.y - p.groups) * 4 * THREADS;
+    const float* x = p.logits + static_cast<int64_t>(bh) * p.groups * p.pitch;
+    float* score = c.score + static_cast<int64_t>(bh) * c.slots;
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f}, old[4];
+    int at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        at[i] = s0 + tid + i * THREADS;
+        at[i] = at[i] < n ? at[i] : n - 1;
+        old[i] = score[at[i]];
     }
-    const int slot = blockIdx.y * THREADS + tid;
-    if (slot < n) {
-        const float* x = p.logits + static_cast<int64_t>(bh) * p.groups * c.slots + slot;
-        float w = 0.0f;
-        for (int g = 0; g < p.groups; ++g) w += __builtin_amdgcn_exp2f(x[static_cast<int64_t>(g) * c.slots] - lse[g]);
-        float* score = c.score + static_cast<int64_t>(bh) * c.slots + slot;
-        *score = (slot == to ? 0.0f : *score) + w;
+#pragma unroll 4
+    for (int g = 0; g < p.groups; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(x[static_cast<int64_t>(g) * p.pitch + at[i]] - lse[g]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (s0 + tid + i * THREADS < n) score[at[i]] = (at[i] == to ? 0.0f : old[i]) + w[i];
+    if (s0 == 0 && tid == 0) {
+        c.position[static_cast<int64_t>(bh) * c.slots + to] = token;
+        c.count[bh] = n;
+        if (h == 0) c.length[b] = token + 1;
     }
 }
 
 struct Plan {
-    int splits, span;
-    size_t logits, partial, plan;
+    int splits, span, pitch;
+    size_t logits, partial, stats, plan;
+    size_t total() const { return logits + partial + stats + plan; }
 };
 
-Plan make_plan(int batch, int q_heads, int kv_heads, int slots, int head_dim, int cus) {
+Plan make_plan(int batch, int q_heads, int kv_heads, int slots, int head_dim) {
     Plan r;
-    const int groups = q_heads / kv_heads;
-    const int64_t rows = static_cast<int64_t>(batch) * kv_heads;
-    static const int per = getenv("ECO_HH") ? atoi(getenv("ECO_HH")) : 2;
-    int64_t splits = (per * static_cast<int64_t>(cus) + rows - 1) / rows;
+    const int64_t groups = q_heads / kv_heads, rows = static_cast<int64_t>(batch) * kv_heads;
+    // as many workgroups as are resident at once on 256 CUs: one per CU at head dim 256 (its tiles fill the LDS), two below
+    // (16 rows of 16 heads and 4096 slots of 256 channels: 177 us at one, 182 at two, 198 at four; 32 rows of 8 heads and 2048
+    // of 128: 59 at one, 58 at two, 61 at four, 66 at six), but at least 128 slots (a step of the four waves) to each
+    const int64_t per_cu = head_dim == 256 ? 1 : 2;
+    int64_t splits = (per_cu * 256 + rows - 1) / rows;
     const int64_t most = (slots + 127) / 128;
     splits = splits > most ? most : splits;
     r.span = static_cast<int>(((slots + splits - 1) / splits + 127) / 128 * 128);
     r.splits = (slots + r.span - 1) / r.span;
+    r.pitch = (slots + 3) / 4 * 4;
     auto align = [](size_t x) { return (x + 255) / 256 * 256; };
-    r.logits = align(sizeof(float) * rows * groups * slots);
-    r.partial = align(sizeof(float) * rows * r.splits * groups * (head_dim + 2));
+    r.logits = align(sizeof(float) * rows * groups * r.pitch);
+    r.partial = align(sizeof(float) * rows * r.splits * groups * head_dim);
+    r.stats = align(sizeof(float) * rows * r.splits * groups * 2);
     r.plan = align(sizeof(int32_t) * rows * 4);
     return r;
 }
@@ -363,12 +404,11 @@ Plan make_plan(int batch, int q_heads, int kv_heads, int slots, int head_dim, in
 template <int D, int FMT>
 int launch(const HeavyParams& p, hipStream_t stream) {
     const BudgetCache& c = p.cache;
-    const int rows = c.batch * c.kv_heads;
-    hipLaunchKernelGGL((heavy_attend_kernel<D, FMT>), dim3(rows, p.splits, ceil_div(p.groups, 16)), dim3(THREADS), 0,
-                       stream, p);
+    const dim3 grid(c.batch * c.kv_heads, p.splits, ceil_div(p.groups, 16));
+    hipLaunchKernelGGL((heavy_attend_kernel<D, FMT>), grid, dim3(THREADS), 0, stream, p);
     if (int rc = check_launch("heavy_attend_kernel")) return rc;
-    hipLaunchKernelGGL((heavy_merge_kernel<D, FMT>), dim3(rows, ceil_div(c.slots, THREADS)), dim3(THREADS), 0, stream,
-                       p);
+    hipLaunchKernelGGL((heavy_merge_kernel<D, FMT>), dim3(grid.x, p.groups + ceil_div(c.slots, 4 * THREADS)), dim3(THREADS),
+                       0, stream, p);
     return check_launch("heavy_merge_kernel");
 }
 
@@ -381,22 +421,22 @@ int launch_dim(const HeavyParams& p, hipStream_t stream) {
 
 }  // namespace
 
-size_t heavy_hitter_workspace(int batch, int q_heads, int kv_heads, int slots, int head_dim, int cus) {
-    const Plan r = make_plan(batch, q_heads, kv_heads, slots, head_dim, cus);
-    return r.logits + r.partial + r.plan;
+size_t heavy_hitter_workspace(int batch, int q_heads, int kv_heads, int slots, int head_dim) {
+    return make_plan(batch, q_heads, kv_heads, slots, head_dim).total();
 }
 
-int heavy_hitter_decode(HeavyParams p, int format, void* workspace, size_t workspace_bytes, int cus,
-                        hipStream_t stream) {
+int heavy_hitter_decode(HeavyParams p, int format, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     const BudgetCache& c = p.cache;
-    const Plan r = make_plan(c.batch, p.q_heads, c.kv_heads, c.slots, c.head_dim, cus);
-    if (workspace_bytes < r.logits + r.partial + r.plan) return fail("heavy-hitter decode: the workspace is too small");
+    const Plan r = make_plan(c.batch, p.q_heads, c.kv_heads, c.slots, c.head_dim);
+    if (workspace_bytes < r.total()) return fail("heavy-hitter decode: the workspace is too small");
     uint8_t* w = static_cast<uint8_t*>(workspace);
     p.logits = reinterpret_cast<float*>(w);
     p.partial = reinterpret_cast<float*>(w + r.logits);
-    p.plan = reinterpret_cast<int32_t*>(w + r.logits + r.partial);
+    p.stats = reinterpret_cast<float*>(w + r.logits + r.partial);
+    p.plan = reinterpret_cast<int32_t*>(w + r.logits + r.partial + r.stats);
     p.splits = r.splits;
     p.span = r.span;
+    p.pitch = r.pitch;
     return format == BF16 ? launch_dim<BF16>(p, stream) : launch_dim<FP16>(p, stream);
 }
 

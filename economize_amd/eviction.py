@@ -11,7 +11,7 @@ decode that evicts nothing more.
 
 from __future__ import annotations
 
-import math
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -20,7 +20,7 @@ from . import _lib
 from .decode import sinks_operand
 from .errors import ConfigError
 from .gathered import GatheredKV
-from .prompt import DTYPES, Rows, operand, row_bounds, strides_of
+from .prompt import DTYPES, Rows, check_out, operand, row_bounds
 
 __all__ = ["HeavyHitterCache", "evict_prompt", "heavy_hitter_attention"]
 
@@ -66,6 +66,22 @@ class HeavyHitterCache:
         return self.keys.shape[2]
 
     def check(self) -> None:
+        """Refuses fields that do not fit together (every call looks: they may be replaced)."""
+        keys, values, score, position = self.keys, self.values, self.score, self.position
+        count, length = self.count, self.length
+        shape, dtype, device = keys.shape, keys.dtype, keys.device
+        if (len(shape) == 4 and shape[3] in (64, 128, 256) and dtype in DTYPES and values.dtype == dtype
+                and values.shape == shape and score.shape == shape[:3] and position.shape == shape[:3]
+                and count.shape == shape[:2] and length.shape == shape[:1] and score.dtype == torch.float32
+                and position.dtype == count.dtype == length.dtype == torch.int32
+                and 0 < self.recent <= shape[2] - self.first <= shape[2] and 0 not in shape
+                and device == values.device == score.device == position.device == count.device == length.device
+                and keys.is_contiguous() and values.is_contiguous() and score.is_contiguous()
+                and position.is_contiguous() and count.is_contiguous() and length.is_contiguous()):
+            return
+        self._refuse()
+
+    def _refuse(self) -> None:
         if self.keys.dim() != 4 or self.keys.dtype not in DTYPES:
             raise ConfigError(f"a heavy-hitter cache holds bf16 or fp16 keys [B, Hkv, budget, D], got {self.keys.dtype} "
                               f"{tuple(self.keys.shape)}")
@@ -74,14 +90,16 @@ class HeavyHitterCache:
             raise ConfigError(f"a heavy-hitter cache needs at least one row, head and slot, got {shape}")
         if dim not in (64, 128, 256):
             raise ConfigError(f"a heavy-hitter cache takes head dims 64, 128 and 256, not {dim}")
+        device = self.keys.device
+        slots, rows = shape[:3], shape[:2]
         for name, t, dtype, want in (("keys", self.keys, self.keys.dtype, shape),
                                      ("values", self.values, self.keys.dtype, shape),
-                                     ("score", self.score, torch.float32, shape[:3]),
-                                     ("position", self.position, torch.int32, shape[:3]),
-                                     ("count", self.count, torch.int32, shape[:2]),
-                                     ("length", self.length, torch.int32, shape[:1])):
-            if t.dtype != dtype or tuple(t.shape) != want or not t.is_contiguous() or t.device != self.keys.device:
-                raise ConfigError(f"{name} must be contiguous {dtype} {list(want)} on {self.keys.device}")
+                                     ("score", self.score, torch.float32, slots),
+                                     ("position", self.position, torch.int32, slots),
+                                     ("count", self.count, torch.int32, rows),
+                                     ("length", self.length, torch.int32, (batch,))):
+            if t.dtype != dtype or t.shape != want or not t.is_contiguous() or t.device != device:
+                raise ConfigError(f"{name} must be contiguous {dtype} {list(want)} on {device}")
         if self.recent < 1 or self.first < 0 or self.recent + self.first > budget:
             raise ConfigError(f"need recent >= 1, first >= 0 and recent + first <= budget, got {self.recent}, {self.first} "
                               f"and {budget}")
@@ -132,12 +150,17 @@ def evict_prompt(cache: HeavyHitterCache, key: torch.Tensor, value: torch.Tensor
         raise ConfigError(f"{sequences} sequences for a cache of {batch} rows")
     if tokens == 0:
         return cache.reset()
-    key, value = operand(key), operand(value)
-    with _lib.on(device):
-        _lib.call("eco_evict_prompt", key.data_ptr(), value.data_ptr(), *strides_of(key), *strides_of(value),
-                  mass.data_ptr(), mass.stride(0) if kv_heads > 1 else tokens, begin, end, tokens,
-                  tokens if max_seqlen is None else min(int(max_seqlen), tokens), *cache._pointers(), batch, kv_heads,
-                  budget, head_dim, int(cache.recent), int(cache.first), _lib.stream_of(device))
+    key, k_at, sk_t, sk_h = operand(key)
+    value, v_at, sv_t, sv_h = operand(value)
+    _lib.call_on(device, "eco_evict_prompt", k_at, v_at, sk_t, sk_h, sv_t, sv_h, mass.data_ptr(),
+                 mass.stride(0) if kv_heads > 1 else tokens, begin, end, tokens,
+                 tokens if max_seqlen is None else min(int(max_seqlen), tokens), *cache._pointers(), batch, kv_heads, budget,
+                 head_dim, cache.recent, cache.first)
+
+
+@functools.lru_cache(maxsize=1024)
+def _step_workspace(*sizes: int) -> int:
+    return _lib.lib().eco_heavy_hitter_workspace_size(*sizes)
 
 
 def heavy_hitter_attention(cache: HeavyHitterCache, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -168,27 +191,26 @@ def heavy_hitter_attention(cache: HeavyHitterCache, query: torch.Tensor, key: to
     q_heads = query.shape[1]
     if q_heads % kv_heads:
         raise ConfigError(f"{q_heads} query heads are not a multiple of {kv_heads} KV heads")
-    for name, t in (("keys", key), ("values", value)):
-        if tuple(t.shape) != (batch, kv_heads, head_dim):
-            raise ConfigError(f"the new {name} must be [{batch}, {kv_heads}, {head_dim}], got {tuple(t.shape)}")
-    for t in (query, key, value):
-        if t.dtype != cache.keys.dtype:
-            raise ConfigError(f"a step of {t.dtype} over a cache of {cache.keys.dtype}")
-    sinks = sinks_operand(sinks, q_heads)
-    if sinks is not None and sinks.device != device:
-        raise ConfigError(f"sinks on {sinks.device}, the queries on {device}")
+    want, dtype = (batch, kv_heads, head_dim), cache.keys.dtype
+    if key.shape != want or value.shape != want:
+        raise ConfigError(f"the new keys and values must be {list(want)}, got {tuple(key.shape)} and {tuple(value.shape)}")
+    if query.dtype != dtype or key.dtype != dtype or value.dtype != dtype:
+        raise ConfigError(f"a step of {query.dtype} queries, {key.dtype} keys and {value.dtype} values over a cache of {dtype}")
+    if sinks is not None:
+        sinks = sinks_operand(sinks, q_heads)
+        if sinks.device != device:
+            raise ConfigError(f"sinks on {sinks.device}, the queries on {device}")
     if out is None:
         out = torch.empty(batch, q_heads, head_dim, dtype=query.dtype, device=device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or operand(out) is not out:
-        raise ConfigError("out must be [B, Hq, D] in the query's dtype on its device, channels contiguous and rows on 16 "
-                          "bytes")
-    query, key, value = operand(query), operand(key), operand(value)
-    with _lib.on(device):
-        need = int(_lib.lib().eco_heavy_hitter_workspace_size(batch, q_heads, kv_heads, budget, head_dim))
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        _lib.call("eco_heavy_hitter_decode", query.data_ptr(), _lib.fmt(query.dtype), *strides_of(query), key.data_ptr(),
-                  value.data_ptr(), *strides_of(key), *strides_of(value), _lib.ptr(sinks), *cache._pointers(),
-                  out.data_ptr(), *strides_of(out), batch, q_heads, kv_heads, budget, head_dim, int(cache.recent),
-                  int(cache.first), float(1 / math.sqrt(head_dim) if scale is None else scale), float(softcap or 0.0),
-                  ws.data_ptr(), need, _lib.stream_of(device))
+        at, so_b, so_h = out.data_ptr(), q_heads * head_dim, head_dim
+    else:
+        at, so_b, so_h = check_out(out, query, "[B, Hq, D]")
+    query, q_at, sq_b, sq_h = operand(query)
+    key, k_at, sk_b, sk_h = operand(key)
+    value, v_at, sv_b, sv_h = operand(value)
+    need = _step_workspace(batch, q_heads, kv_heads, budget, head_dim)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.call_on(device, "eco_heavy_hitter_decode", q_at, _lib.fmt(query.dtype), sq_b, sq_h, k_at, v_at, sk_b, sk_h, sv_b,
+                 sv_h, _lib.ptr(sinks), *cache._pointers(), at, so_b, so_h, batch, q_heads, kv_heads, budget, head_dim,
+                 cache.recent, cache.first, head_dim ** -0.5 if scale is None else scale, softcap or 0.0, ws.data_ptr(), need)
     return out

@@ -11,6 +11,7 @@ batch). ``max_seqlen`` is the longest one (it sizes the launch; the number of ro
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Union
 
@@ -26,11 +27,13 @@ __all__ = ["Rows", "attention_mass", "prompt_attention"]
 Rows = Union[torch.Tensor, tuple[torch.Tensor, torch.Tensor]]
 
 DTYPES = (torch.bfloat16, torch.float16)
+#: Strides the kernels take, in elements: a tile's rows lie within 32 bits of its first one.
+STRIDE_LIMIT = 1 << 24
 
 
-def row_bounds(rows: Rows, device: torch.device) -> tuple[torch.Tensor, int, int, int]:
-    """A tensor that keeps the bounds alive, the addresses of every sequence's first and past-the-end row, and how many
-    sequences there are."""
+def row_bounds(rows: Rows, device: torch.device) -> tuple[object, int, int, int]:
+    """What keeps the bounds alive, the addresses of every sequence's first and past-the-end row, and how many sequences
+    there are."""
     if torch.is_tensor(rows):
         if rows.dtype != torch.int32 or rows.dim() != 1 or rows.numel() < 2 or rows.stride(0) != 1:
             raise ConfigError("cu_seqlens must be contiguous int32 [sequences + 1] with at least one sequence")
@@ -44,22 +47,33 @@ def row_bounds(rows: Rows, device: torch.device) -> tuple[torch.Tensor, int, int
             raise ConfigError(f"begin and end must be contiguous int32 [sequences] on {device}")
     if begin.numel() != end.numel():
         raise ConfigError(f"{begin.numel()} sequences begin, {end.numel()} end")
-    return begin, begin.data_ptr(), end.data_ptr(), begin.numel()
+    return rows, begin.data_ptr(), end.data_ptr(), begin.numel()
 
 
-def operand(x: torch.Tensor) -> torch.Tensor:
-    """``x`` ``[..., D]`` as the kernels read it: unit channel stride, base and other strides whole 16 bytes from 0 to below
-    2^24 elements (a copy only when it is not)."""
-    es = x.element_size()
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
-            n == 1 or (0 <= s < 1 << 24 and (s * es) % 16 == 0) for n, s in zip(x.shape[:-1], x.stride()[:-1])):
-        return x
-    return x.contiguous()
+def operand(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """``x`` ``[A, B, D]`` of 16-bit elements as the kernels read it, its address and its first two strides: unit channel
+    stride, address and strides whole 16 bytes, strides from 0 to below :data:`STRIDE_LIMIT` (a copy only when it is not; the
+    stride of an axis of one entry is not used and given as 0)."""
+    a, b, c = x.stride()
+    at = x.data_ptr()
+    if c == 1 and not (at & 15 or a & 7 or b & 7) and 0 <= a < STRIDE_LIMIT and 0 <= b < STRIDE_LIMIT:
+        return x, at, a, b
+    a, b = (0 if n <= 1 else s for n, s in zip(x.shape, (a, b)))
+    if c == 1 and not (at & 15 or a & 7 or b & 7) and 0 <= a < STRIDE_LIMIT and 0 <= b < STRIDE_LIMIT:
+        return x, at, a, b
+    copy = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    copy.copy_(x)
+    return copy, copy.data_ptr(), copy.stride(0), copy.stride(1)
 
 
-def strides_of(x: torch.Tensor) -> tuple[int, int]:
-    """The first two strides; that of an axis of one entry is not used and may be anything, so it is given as 0."""
-    return tuple(0 if n == 1 else s for n, s in zip(x.shape[:2], x.stride()[:2]))
+def check_out(out: torch.Tensor, like: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """The address and strides of an output buffer the kernels can write."""
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ConfigError(f"out must be {what} in the query's dtype on its device")
+    same, at, a, b = operand(out)
+    if same is not out:
+        raise ConfigError(f"out must be {what}, channels contiguous and rows on 16 bytes")
+    return at, a, b
 
 
 def _check(what: str, query: torch.Tensor, key: torch.Tensor) -> None:
@@ -70,6 +84,28 @@ def _check(what: str, query: torch.Tensor, key: torch.Tensor) -> None:
         raise ConfigError(f"{what} takes bf16 or fp16 queries and keys of one dtype, got {query.dtype} and {key.dtype}")
     if key.shape[1] == 0 or query.shape[1] % key.shape[1] or query.shape[1] == 0:
         raise ConfigError(f"{query.shape[1]} query heads are not a multiple of {key.shape[1]} KV heads")
+
+
+@functools.lru_cache(maxsize=1024)
+def _prompt_workspace(*sizes: int) -> int:
+    return _lib.lib().eco_prompt_attention_workspace_size(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _mass_workspace(*sizes: int) -> int:
+    return _lib.lib().eco_attention_mass_workspace_size(*sizes)
+
+
+def _sequences(cu_seqlens: Rows, cu_seqlens_k: Rows | None, tokens: int, keys: int, device: torch.device) -> tuple:
+    bounds = row_bounds(cu_seqlens, device)
+    if cu_seqlens_k is None:
+        if keys != tokens:
+            raise ConfigError(f"{keys} keys for {tokens} queries need cu_seqlens_k")
+        return bounds, bounds
+    bounds_k = row_bounds(cu_seqlens_k, device)
+    if bounds_k[3] != bounds[3]:
+        raise ConfigError(f"{bounds[3]} sequences of queries, {bounds_k[3]} of keys")
+    return bounds, bounds_k
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: Rows,
@@ -102,40 +138,37 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if value.shape != key.shape or value.dtype != key.dtype:
         raise ConfigError(f"values {tuple(value.shape)} {value.dtype} do not match the keys {tuple(key.shape)} {key.dtype}")
     tokens, q_heads, head_dim = query.shape
-    keep_q, q_begin, q_end, sequences = row_bounds(cu_seqlens, device)
-    keep_k, k_begin, k_end, k_sequences = (keep_q, q_begin, q_end, sequences) if cu_seqlens_k is None else \
-        row_bounds(cu_seqlens_k, device)
-    if k_sequences != sequences:
-        raise ConfigError(f"{sequences} sequences of queries, {k_sequences} of keys")
-    if cu_seqlens_k is None and key.shape[0] != tokens:
-        raise ConfigError(f"{key.shape[0]} keys for {tokens} queries need cu_seqlens_k")
-    sinks = sinks_operand(sinks, q_heads)
-    if sinks is not None and sinks.device != device:
-        raise ConfigError(f"sinks on {sinks.device}, the queries on {device}")
+    keys, kv_heads, _ = key.shape
+    (keep, q_begin, q_end, sequences), (keep_k, k_begin, k_end, _) = _sequences(cu_seqlens, cu_seqlens_k, tokens, keys,
+                                                                                device)
+    if sinks is not None:
+        sinks = sinks_operand(sinks, q_heads)
+        if sinks.device != device:
+            raise ConfigError(f"sinks on {sinks.device}, the queries on {device}")
     fill = out is None
-    if out is None:
+    if fill:
         out = torch.empty(tokens, q_heads, head_dim, dtype=query.dtype, device=device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or operand(out) is not out:
-        raise ConfigError("out must be [T, Hq, D] in the query's dtype on its device, channels contiguous and rows on 16 "
-                          "bytes")
-    lse = torch.empty(q_heads, tokens, dtype=torch.float32, device=device) if return_lse else None
-    if return_lse and not fill:
-        lse.fill_(-math.inf)
-    query, key, value = operand(query), operand(key), operand(value)
-    max_q = tokens if max_seqlen is None else min(int(max_seqlen), tokens)
-    max_k = key.shape[0] if max_seqlen_k is None else min(int(max_seqlen_k), key.shape[0])
-    if cu_seqlens_k is None and max_seqlen_k is None:
-        max_k = max_q
-    with _lib.on(device):
-        need = _lib.lib().eco_prompt_attention_workspace_size(sequences, tokens, max_q, max_k, q_heads, key.shape[1],
-                                                              head_dim)
+        at, so_t, so_h = out.data_ptr(), q_heads * head_dim, head_dim
+    else:
+        at, so_t, so_h = check_out(out, query, "[T, Hq, D]")
+    lse = None
+    if return_lse:
+        lse = torch.empty(q_heads, tokens, dtype=torch.float32, device=device)
+        if not fill:
+            lse.fill_(-math.inf)
+    if tokens:
+        query, q_at, sq_t, sq_h = operand(query)
+        key, k_at, sk_t, sk_h = operand(key)
+        value, v_at, sv_t, sv_h = operand(value)
+        max_q = tokens if max_seqlen is None else min(int(max_seqlen), tokens)
+        max_k = min(int(max_seqlen_k), keys) if max_seqlen_k is not None else max_q if cu_seqlens_k is None else keys
+        need = _prompt_workspace(sequences, tokens, max_q, max_k, q_heads, kv_heads, head_dim)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        _lib.call(
-            "eco_prompt_attention", query.data_ptr(), _lib.fmt(query.dtype), *strides_of(query), key.data_ptr(),
-            value.data_ptr(), *strides_of(key), *strides_of(value), q_begin, q_end, k_begin, k_end, sequences, tokens,
-            key.shape[0], max_q, max_k, _lib.ptr(sinks), out.data_ptr(), *strides_of(out), _lib.ptr(lse), tokens,
-            int(fill), q_heads, key.shape[1], head_dim, float(1 / math.sqrt(head_dim) if scale is None else scale),
-            float(softcap or 0.0), _lib.ptr(ws), need, _lib.stream_of(device))
+        _lib.call_on(
+            device, "eco_prompt_attention", q_at, _lib.fmt(query.dtype), sq_t, sq_h, k_at, v_at, sk_t, sk_h, sv_t, sv_h,
+            q_begin, q_end, k_begin, k_end, sequences, tokens, keys, max_q, max_k, _lib.ptr(sinks), at, so_t, so_h,
+            _lib.ptr(lse), tokens, fill, q_heads, kv_heads, head_dim, head_dim ** -0.5 if scale is None else scale,
+            softcap or 0.0, _lib.ptr(ws), need)
     return (out, lse) if return_lse else out
 
 
@@ -161,34 +194,26 @@ def attention_mass(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu
         raise ConfigError(f"lse must be fp32 [{q_heads}, {tokens}] with contiguous rows apart")
     if window is not None and (isinstance(window, bool) or int(window) != window or window < 1):
         raise ConfigError(f"window must be a positive integer or None, got {window!r}")
-    keep_q, q_begin, q_end, sequences = row_bounds(cu_seqlens, device)
-    keep_k, k_begin, k_end, k_sequences = (keep_q, q_begin, q_end, sequences) if cu_seqlens_k is None else \
-        row_bounds(cu_seqlens_k, device)
-    if k_sequences != sequences:
-        raise ConfigError(f"{sequences} sequences of queries, {k_sequences} of keys")
-    keys, kv_heads = key.shape[:2]
-    if cu_seqlens_k is None and keys != tokens:
-        raise ConfigError(f"{keys} keys for {tokens} queries need cu_seqlens_k")
+    keys, kv_heads, _ = key.shape
+    (keep, q_begin, q_end, sequences), (keep_k, k_begin, k_end, _) = _sequences(cu_seqlens, cu_seqlens_k, tokens, keys,
+                                                                                device)
     fill = out is None
-    if out is None:
+    if fill:
         out = torch.empty(kv_heads, keys, dtype=torch.float32, device=device)
     elif out.dtype != torch.float32 or tuple(out.shape) != (kv_heads, keys) or out.device != device or \
             (keys > 1 and out.stride(1) != 1) or (kv_heads > 1 and out.stride(0) < keys):
         raise ConfigError(f"out must be fp32 [{kv_heads}, {keys}] with contiguous rows apart on {device}")
-    query, key = operand(query), operand(key)
-    max_q = tokens if max_seqlen is None else min(int(max_seqlen), tokens)
-    max_k = keys if max_seqlen_k is None else min(int(max_seqlen_k), keys)
-    if cu_seqlens_k is None and max_seqlen_k is None:
-        max_k = max_q
-    window = min(int(window or 0), 0x7fffffff)
-    with _lib.on(device):
-        need = _lib.lib().eco_attention_mass_workspace_size(max_q, keys, window, q_heads, kv_heads)
+    if keys:
+        query, q_at, sq_t, sq_h = operand(query)
+        key, k_at, sk_t, sk_h = operand(key)
+        max_q = tokens if max_seqlen is None else min(int(max_seqlen), tokens)
+        max_k = min(int(max_seqlen_k), keys) if max_seqlen_k is not None else max_q if cu_seqlens_k is None else keys
+        window = min(int(window or 0), 0x7fffffff)
+        need = _mass_workspace(max_q, keys, window, q_heads, kv_heads)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        _lib.call(
-            "eco_attention_mass", query.data_ptr(), _lib.fmt(query.dtype), *strides_of(query), key.data_ptr(),
-            *strides_of(key), lse.data_ptr(), lse.stride(0) if q_heads > 1 else tokens, q_begin, q_end, k_begin, k_end,
-            sequences, tokens, keys, max_q, max_k, window, out.data_ptr(),
-            out.stride(0) if kv_heads > 1 else keys, int(fill), q_heads, kv_heads, head_dim,
-            float(1 / math.sqrt(head_dim) if scale is None else scale), float(softcap or 0.0), _lib.ptr(ws), need,
-            _lib.stream_of(device))
+        _lib.call_on(
+            device, "eco_attention_mass", q_at, _lib.fmt(query.dtype), sq_t, sq_h, k_at, sk_t, sk_h, lse.data_ptr(),
+            lse.stride(0) if q_heads > 1 else tokens, q_begin, q_end, k_begin, k_end, sequences, tokens, keys, max_q, max_k,
+            window, out.data_ptr(), out.stride(0) if kv_heads > 1 else keys, fill, q_heads, kv_heads, head_dim,
+            head_dim ** -0.5 if scale is None else scale, softcap or 0.0, _lib.ptr(ws), need)
     return out

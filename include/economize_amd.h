@@ -516,7 +516,7 @@ int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, i
  * filled, the slot of least score whose position lies in [first, length[b] - recent] (equal: the lower slot; a NaN is
  * the least); q [B, Hq, D] attends over the filled slots (out [B, Hq, D]); every filled slot's score grows by its weight
  * summed over the query heads of its KV head (the new one's from 0); count and length advance. At most 64 query heads per
- * KV head. The workspace need not be cleared. */
+ * KV head. The workspace need not be cleared. Calls on one cache may not overlap. */
 size_t eco_heavy_hitter_workspace_size(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t slots,
                                        int32_t head_dim);
 int eco_heavy_hitter_decode(const void* q, int32_t format, int64_t sq_b, int64_t sq_h, const void* k, const void* v,
