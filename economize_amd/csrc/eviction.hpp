@@ -41,6 +41,7 @@ struct HeavyParams {
     int q_heads, groups;
     int splits, span;  // parts a row's slots are cut into, slots of a part
     float scale, softcap;
+    int chosen;      // whether a launch before chose the slots (else every workgroup chooses)
     int pitch;       // slots of a row of `logits`: C in whole fours
     float* logits;   // workspace: [B, Hkv, G, pitch]
     float* partial;  // [B, Hkv, splits, G, D]

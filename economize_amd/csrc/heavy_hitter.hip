@@ -10,7 +10,6 @@
 // fixed order: no atomics. (The join by the last part of a row to finish, in the same launch, took as long for 2048 slots of
 // 4 heads, 57.6 us against 55.0, and twice as long for one row of 8192, 83 against 44.)
 
-#include <cstdlib>
 #include "eviction.hpp"
 
 namespace eco {
@@ -47,6 +46,7 @@ __device__ __forceinline__ uint32_t pair16(float a, float b) {
 }
 
 // The slot the new token takes (the same in every workgroup of the row and head).
+template <int THREADS>
 __device__ __forceinline__ int choose_slot(const BudgetCache& c, int bh, int filled, int token, uint64_t* scratch) {
     if (filled < c.slots) return filled;
     const float* score = c.score + static_cast<int64_t>(bh) * c.slots;
@@ -78,8 +78,19 @@ __device__ __forceinline__ int choose_slot(const BudgetCache& c, int bh, int fil
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = best;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) best = scratch[w] < best ? scratch[w] : best;
+    for (int w = 0; w < THREADS / 64; ++w) best = scratch[w] < best ? scratch[w] : best;
     return static_cast<int>(static_cast<uint32_t>(best));
+}
+
+constexpr int CHOOSERS = 1024;
+
+__global__ __launch_bounds__(CHOOSERS) void heavy_choose_kernel(HeavyParams p) {
+    __shared__ uint64_t scratch[CHOOSERS / 64];
+    const int bh = blockIdx.x;
+    int filled = p.cache.count[bh];
+    filled = filled < 0 ? 0 : (filled > p.cache.slots ? p.cache.slots : filled);
+    const int to = choose_slot<CHOOSERS>(p.cache, bh, filled, p.cache.length[bh / p.cache.kv_heads], scratch);
+    if (threadIdx.x == 0) p.plan[4 * static_cast<int64_t>(bh)] = to;
 }
 
 // 32 slots of one wave in LDS, in chunks of 16 bytes; the swizzles spread the rows of one fragment read (16 rows of 16
@@ -143,11 +154,11 @@ __global__ __launch_bounds__(THREADS, (D == 256 ? 1 : 2)) void heavy_attend_kern
     for (int i = 0; i < KS; ++i) qf[i] = *reinterpret_cast<const uint4*>(qp + 32 * i);
     const uint16_t* new_k = p.k + b * p.sk_b + h * p.sk_h;
     const uint16_t* new_v = p.v + b * p.sv_b + h * p.sv_h;
-    const int to = choose_slot(c, bh, filled, token, scratch);
+    int32_t* plan = p.plan + 4 * static_cast<int64_t>(bh);
+    const int to = p.chosen ? plan[0] : choose_slot<THREADS>(c, bh, filled, token, scratch);
     const int n = filled < c.slots ? filled + 1 : c.slots;
     if (split == 0 && block == 0 && tid == 0) {
-        int32_t* plan = p.plan + 4 * static_cast<int64_t>(bh);
-        plan[0] = to;
+        if (!p.chosen) plan[0] = to;
         plan[1] = n;
         plan[2] = token;
     }
@@ -405,6 +416,10 @@ template <int D, int FMT>
 int launch(const HeavyParams& p, hipStream_t stream) {
     const BudgetCache& c = p.cache;
     const dim3 grid(c.batch * c.kv_heads, p.splits, ceil_div(p.groups, 16));
+    if (p.chosen) {
+        hipLaunchKernelGGL(heavy_choose_kernel, dim3(grid.x), dim3(CHOOSERS), 0, stream, p);
+        if (int rc = check_launch("heavy_choose_kernel")) return rc;
+    }
     hipLaunchKernelGGL((heavy_attend_kernel<D, FMT>), grid, dim3(THREADS), 0, stream, p);
     if (int rc = check_launch("heavy_attend_kernel")) return rc;
     hipLaunchKernelGGL((heavy_merge_kernel<D, FMT>), dim3(grid.x, p.groups + ceil_div(c.slots, 4 * THREADS)), dim3(THREADS),
@@ -437,6 +452,10 @@ int heavy_hitter_decode(HeavyParams p, int format, void* workspace, size_t works
     p.splits = r.splits;
     p.span = r.span;
     p.pitch = r.pitch;
+    // Every workgroup reading all scores and positions of its row costs less than a launch until there are many of both (one
+    // row of 8 heads: 8192 slots 17 us either way, 32768 slots 36 us against 40, 131072 slots 129 against 158; 32 rows of 2048
+    // slots 60 against 57).
+    p.chosen = c.slots >= 16384;
     return format == BF16 ? launch_dim<BF16>(p, stream) : launch_dim<FP16>(p, stream);
 }
 

@@ -33,7 +33,7 @@ def check_evicted(cache, k, v, mass, cu) -> None:
             assert torch.equal(cache.score[b, h, :n].view(torch.int32), mass[h, at].view(torch.int32))
 
 
-LENGTHS = [[0, 1, 63], [64, 65], [66, 200, 64], [1000, 4096, 4097], [5000]]
+LENGTHS = [[0, 1, 63], [64, 65], [66, 200, 64], [1000, 4096, 4097], [5000], [16384, 16385, 300], [40000]]
 
 
 @pytest.mark.parametrize("lens", LENGTHS, ids=lambda x: "-".join(map(str, x)))
@@ -209,6 +209,13 @@ def test_slots_past_the_count_are_not_read() -> None:
         cache.position[b, :, n:] = -7
     for _ in range(2):
         step_and_check(cache, *new_token(gen, 3, heads, 128, BF16))
+
+
+def test_a_step_over_many_slots() -> None:
+    """Enough slots that a launch of its own chooses the new token's."""
+    cache, gen = make_cache(21, 1, (4, 2), 64, BF16, 16400, 900, 4, [30000])
+    for _ in range(2):
+        step_and_check(cache, *new_token(gen, 1, (4, 2), 64, BF16))
 
 
 def test_strided_step_and_out() -> None:
