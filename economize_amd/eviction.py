@@ -65,23 +65,14 @@ class HeavyHitterCache:
     def budget(self) -> int:
         return self.keys.shape[2]
 
-    def check(self) -> None:
-        """Refuses fields that do not fit together (every call looks: they may be replaced)."""
-        keys, values, score, position = self.keys, self.values, self.score, self.position
-        count, length = self.count, self.length
-        shape, dtype, device = keys.shape, keys.dtype, keys.device
-        if (len(shape) == 4 and shape[3] in (64, 128, 256) and dtype in DTYPES and values.dtype == dtype
-                and values.shape == shape and score.shape == shape[:3] and position.shape == shape[:3]
-                and count.shape == shape[:2] and length.shape == shape[:1] and score.dtype == torch.float32
-                and position.dtype == count.dtype == length.dtype == torch.int32
-                and 0 < self.recent <= shape[2] - self.first <= shape[2] and 0 not in shape
-                and device == values.device == score.device == position.device == count.device == length.device
-                and keys.is_contiguous() and values.is_contiguous() and score.is_contiguous()
-                and position.is_contiguous() and count.is_contiguous() and length.is_contiguous()):
-            return
-        self._refuse()
+    def __setattr__(self, name: str, value: object) -> None:
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_checked", False)  # (a field replaced: the next call looks at all of them again)
 
-    def _refuse(self) -> None:
+    def check(self) -> None:
+        """Refuses fields that do not fit together, once after any of them was set."""
+        if self._checked:
+            return
         if self.keys.dim() != 4 or self.keys.dtype not in DTYPES:
             raise ConfigError(f"a heavy-hitter cache holds bf16 or fp16 keys [B, Hkv, budget, D], got {self.keys.dtype} "
                               f"{tuple(self.keys.shape)}")
@@ -103,6 +94,7 @@ class HeavyHitterCache:
         if self.recent < 1 or self.first < 0 or self.recent + self.first > budget:
             raise ConfigError(f"need recent >= 1, first >= 0 and recent + first <= budget, got {self.recent}, {self.first} "
                               f"and {budget}")
+        object.__setattr__(self, "_checked", True)
 
     def reset(self) -> None:
         self.count.zero_()

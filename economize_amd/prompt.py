@@ -35,7 +35,7 @@ def row_bounds(rows: Rows, device: torch.device) -> tuple[object, int, int, int]
     """What keeps the bounds alive, the addresses of every sequence's first and past-the-end row, and how many sequences
     there are."""
     if torch.is_tensor(rows):
-        if rows.dtype != torch.int32 or rows.dim() != 1 or rows.numel() < 2 or rows.stride(0) != 1:
+        if rows.dtype is not torch.int32 or rows.dim() != 1 or rows.numel() < 2 or rows.stride(0) != 1:
             raise ConfigError("cu_seqlens must be contiguous int32 [sequences + 1] with at least one sequence")
         if rows.device != device:
             raise ConfigError(f"cu_seqlens on {rows.device}, the queries on {device}")
@@ -102,7 +102,7 @@ def _sequences(cu_seqlens: Rows, cu_seqlens_k: Rows | None, tokens: int, keys: i
         if keys != tokens:
             raise ConfigError(f"{keys} keys for {tokens} queries need cu_seqlens_k")
         return bounds, bounds
-    bounds_k = row_bounds(cu_seqlens_k, device)
+    bounds_k = bounds if cu_seqlens_k is cu_seqlens else row_bounds(cu_seqlens_k, device)
     if bounds_k[3] != bounds[3]:
         raise ConfigError(f"{bounds[3]} sequences of queries, {bounds_k[3]} of keys")
     return bounds, bounds_k
