@@ -42,8 +42,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
     }
     int pair, slot;
     if (!work_of(p.order, blockIdx.x, pair, slot)) return;
-    const int part = slot % p.parts, first = slot / p.parts, stride = p.order.tiles / p.parts;
-    const int s = pair / p.kv_heads, kvh = pair % p.kv_heads;
+    const int first = p.per_part(slot), part = slot - first * p.parts, stride = p.order.tiles / p.parts;
+    const int s = p.per_kv(pair), kvh = pair - s * p.kv_heads;
     const Sequence seq = sequence_of(p.rows, s);
     const int tiles = (seq.nk + KEYS - 1) / KEYS;
     const int offset = seq.nk - seq.nq;
@@ -210,6 +210,8 @@ int launch(MassParams p, int max_queries, int max_keys, hipStream_t stream) {
     const int64_t bytes = static_cast<int64_t>(max_queries) * p.groups * D * 2;
     p.order = work_order(p.rows.sequences, p.kv_heads, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
     p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
+    p.per_kv = Divisor(p.kv_heads);
+    p.per_part = Divisor(p.parts);
     const int fill = p.fill ? 8 : 0;
     p.fill = fill;
     const dim3 grid(static_cast<uint32_t>(p.order.blocks() + fill));

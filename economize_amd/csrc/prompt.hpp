@@ -15,11 +15,23 @@ struct PackedRows {
     int64_t q_rows, k_rows;
 };
 
+// x / by for 0 <= x < 2^31 - by through one product: 2^32 over `by` rounded up gives the quotient or one more.
+struct Divisor {
+    uint32_t by, inverse;
+    Divisor() = default;
+    explicit Divisor(int64_t d) : by(static_cast<uint32_t>(d)), inverse(static_cast<uint32_t>((0x100000000ull + d - 1) / d)) {}
+    __host__ __device__ __forceinline__ int operator()(int x) const {
+        const int q = static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * inverse >> 32);
+        return by == 1 ? x : q - (q * static_cast<int>(by) > x ? 1 : 0);
+    }
+};
+
 // Which (sequence, KV head) pair and which of its tiles a workgroup takes. The tiles of a pair read the same rows, so they
 // run close together: the pairs in `group` at a time, their longest tiles first. Workgroups go to the eight XCDs in turn,
 // each with an L2 of its own: with `pin` a pair stays on one.
 struct WorkOrder {
     int pairs, tiles, group, pin;
+    Divisor whole, full_width, last_width;  // workgroups of a group of pairs; pairs in a group, and in the last one
     int per_xcd() const { return (pairs + 7) / 8; }
     int64_t blocks() const { return static_cast<int64_t>(tiles) * (pin ? 8 * per_xcd() : pairs); }
 };
@@ -39,6 +51,9 @@ inline WorkOrder work_order(int sequences, int kv_heads, int64_t tiles, int64_t 
     // (an odd number: workgroups in turn go to the four shader engines of an XCD, and where only every other pair has
     // tiles left, two of the engines would be idle)
     o.group = static_cast<int>(fit < 1 ? 1 : fit > most ? most : fit - (fit % 2 == 0));
+    o.whole = Divisor(static_cast<int64_t>(o.tiles) * o.group);
+    o.full_width = Divisor(o.group);
+    o.last_width = Divisor((most - 1) % o.group + 1);
     return o;
 }
 
@@ -53,7 +68,7 @@ struct PromptParams {
     int64_t sl_h;
     int fill;  // workgroups that give rows of no sequence out 0 and lse -inf (0: they are left as they are)
     int q_heads, kv_heads, groups, head_dim;
-    uint32_t group_inverse;
+    Divisor per_group, per_kv, per_part;  // over the groups, the KV heads, the row tiles of a part
     WorkOrder order;  // (sequences of more row tiles than the launch holds loop over them)
     int parts;                     // a row tile's keys are cut into up to so many
     float *part_out, *part_stats;  // [parts, q_rows, Hq, D] and [.., 2], of the row tiles that were cut
@@ -76,6 +91,7 @@ struct MassParams {
     int fill;    // workgroups that give keys of no sequence 0 (0: they are left as they are)
     int window;  // only the last `window` queries of a sequence count
     int q_heads, kv_heads, groups, head_dim;
+    Divisor per_kv, per_part;
     WorkOrder order;  // (sequences of more key tiles than the launch holds loop over them)
     int parts;       // a key tile's query heads are cut into so many parts (1, or one per head)
     float* partial;  // [parts, Hkv, k_rows] where parts > 1

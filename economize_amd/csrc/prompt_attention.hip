@@ -65,19 +65,15 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
     int pair, slot;
     if (!work_of(p.order, blockIdx.x, pair, slot)) return;
     // (parts outermost: workgroups without work come last, where they leave no shader engine without any)
-    const int stride = p.order.tiles / p.parts, part = slot / stride, first = slot % stride;
-    const int s = pair / p.kv_heads, kvh = pair % p.kv_heads;
+    const int stride = p.per_part.by, part = p.per_part(slot), first = slot - part * stride;
+    const int s = p.per_kv(pair), kvh = pair - s * p.kv_heads;
     const Sequence seq = sequence_of(p.rows, s);
     const int total = seq.nq * p.groups;  // (below 2^31: the host checks)
     const int tiles = (total + ROWS - 1) / ROWS;
     const int offset = seq.nk - seq.nq;  // query i sees keys <= i + offset
     const uint16_t* kbase = p.k + seq.k0 * p.sk_t + kvh * p.sk_h;
     const uint16_t* vbase = p.v + seq.k0 * p.sv_t + kvh * p.sv_h;
-    // r / groups for 0 <= r < 2^31: the multiplier is 2^32 over the groups rounded up, so the quotient is right or one over
-    auto over_groups = [&](int r) {
-        const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.group_inverse));
-        return p.groups == 1 ? r : q - (q * p.groups > r ? 1 : 0);
-    };
+    auto over_groups = [&](int r) { return p.per_group(r); };
     const float cc = CAP ? 1.0f : p.scale * kLog2e;
     const TileCopy<D, THREADS> kcopy(tid, p.sk_t, true), vcopy(tid, p.sv_t, false);
     // Fragment places in a tile: keys row l % 32, 8 channels from 8 (l / 32); values transposed, rows 4 (l / 32) + l % 16 / 4,
@@ -455,7 +451,9 @@ int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
     const int64_t bytes = static_cast<int64_t>(max_keys) * D * 4;
     p.order = work_order(p.rows.sequences, p.kv_heads, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
     p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
-    p.group_inverse = static_cast<uint32_t>((0x100000000ull + p.groups - 1) / p.groups);
+    p.per_group = Divisor(p.groups);
+    p.per_kv = Divisor(p.kv_heads);
+    p.per_part = Divisor(p.order.tiles / p.parts);
     p.fill = p.fill ? 32 : 0;
     const dim3 grid(static_cast<uint32_t>(p.order.blocks() + p.fill));
     if (p.softcap > 0.0f)

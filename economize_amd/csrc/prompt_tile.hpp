@@ -63,12 +63,13 @@ __device__ __forceinline__ Sequence sequence_of(const PackedRows& r, int s) {
 
 // The pair and the tile (0 the longest) of workgroup id; false where there is none.
 __device__ __forceinline__ bool work_of(const WorkOrder& o, int id, int& pair, int& tile) {
-    const int lanes = o.pin ? 8 : 1, total = o.pin ? (o.pairs + 7) / 8 : o.pairs;
-    const int k = id / lanes, whole = o.tiles * o.group;
-    const int first = k / whole * o.group, within = k % whole;
-    const int width = total - first < o.group ? total - first : o.group;
-    tile = within / width;
-    pair = (first + within % width) * lanes + id % lanes;
+    const int total = o.pin ? (o.pairs + 7) / 8 : o.pairs;
+    const int k = o.pin ? id >> 3 : id;
+    const int group = o.whole(k), first = group * o.group, within = k - group * static_cast<int>(o.whole.by);
+    const bool last = total - first < o.group;
+    tile = last ? o.last_width(within) : o.full_width(within);
+    const int p = first + within - tile * static_cast<int>(last ? o.last_width.by : o.full_width.by);
+    pair = o.pin ? p * 8 + (id & 7) : p;
     return pair < o.pairs;
 }
 
