@@ -6,7 +6,8 @@
 // S = Q K^T puts one key in each lane with 16 of 32 queries in its registers, so a weight is added where it is computed, in
 // fp32 and in a fixed order: no atomics, the same bits every time. The products of 32 queries run while the weights of the
 // 32 before are computed. All tiles of a (sequence, KV head) walk the queries from the last down, so they read the same ones
-// at the same time. Long walks are cut by heads, each a workgroup of its own, summed by mass_sum_kernel.
+// at the same time. Long walks are cut by
+// heads, each a workgroup of its own, summed by mass_sum_kernel.
 
 #include "prompt_tile.hpp"
 
@@ -18,7 +19,7 @@ constexpr int WAVES = 4;
 constexpr int THREADS = WAVES * 64;
 
 template <int D, int FMT, int KT, bool CAP>
-__global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p) {
+__global__ __launch_bounds__(THREADS, KT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5) void attention_mass_kernel(MassParams p) {
     typedef Tile<D> T;
     constexpr int KS = D / 16;
     constexpr int KEYS = WAVES * 32 * KT;
@@ -29,15 +30,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_mass_kernel(MassParams p
     const int col = lane & 31, half = lane >> 5;
     const int work = gridDim.x - p.fill;
     if (static_cast<int>(blockIdx.x) >= work) {  // the last workgroups: keys of no sequence
-        const int workers = p.fill, me = blockIdx.x - work;
-        for (int g = 0; g <= p.rows.sequences; ++g) {
-            int64_t from = g == 0 ? 0 : p.rows.k_end[g - 1];
-            int64_t to = g == p.rows.sequences ? p.rows.k_rows : p.rows.k_begin[g];
-            from = from < 0 ? 0 : from;
-            to = to > p.rows.k_rows ? p.rows.k_rows : to;
-            for (int64_t t = from + me * THREADS + tid; t < to; t += static_cast<int64_t>(workers) * THREADS)
+        for_gaps(p.rows.k_begin, p.rows.k_end, p.rows.sequences, p.rows.k_rows, blockIdx.x - work,
+                 [&](int64_t from, int64_t to, int worker, int workers) {
+            for (int64_t t = from + worker * THREADS + tid; t < to; t += static_cast<int64_t>(workers) * THREADS)
                 for (int h = 0; h < p.kv_heads; ++h) p.mass[h * p.sm_h + t] = 0.0f;
-        }
+        });
         return;
     }
     int pair, slot;
@@ -194,27 +191,25 @@ __global__ __launch_bounds__(256) void mass_sum_kernel(MassParams p) {
     }
 }
 
-constexpr int keys_per_tile(int head_dim) { return WAVES * 32 * (head_dim == 256 ? 1 : 2); }
-
-// Walks of 64 steps and more are cut by heads: their lengths differ up to the whole, and shorter ones even out.
-int parts_of(int max_queries, int groups) {
-    return (static_cast<int64_t>(max_queries) + 63) / 64 * groups >= 64 ? groups : 1;
+// Long walks are cut by heads: their lengths differ up to the whole, and shorter ones even out (one prompt of 500 tokens,
+// 32 heads of 128 on 8: 40 us whole, 16 us cut). A window's walks are as long as each other and only gain from being many
+// (window 256 over 16 x 4200 keys: 151 us whole, 167 cut; window 512 over 30000: 151 and 135).
+int parts_of(int max_queries, bool windowed, int groups) {
+    const int64_t steps = (static_cast<int64_t>(max_queries) + 63) / 64 * groups;
+    return steps >= (windowed ? 32 : 12) ? groups : 1;
 }
 
 template <int D, int FMT, int KT>
 int launch(MassParams p, int max_queries, int max_keys, hipStream_t stream) {
     constexpr int KEYS = WAVES * 32 * KT;
-    static_assert(KEYS == keys_per_tile(D), "one tile size per head dim");
     const int64_t pairs = static_cast<int64_t>(p.rows.sequences) * p.kv_heads;
     const int64_t tiles = (static_cast<int64_t>(max_keys) + KEYS - 1) / KEYS;
     const int64_t bytes = static_cast<int64_t>(max_queries) * p.groups * D * 2;
-    p.order = work_order(p.rows.sequences, p.kv_heads, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
-    p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
+    p.order = work_order(p.rows.sequences, p.kv_heads, tiles, p.parts, bytes);
     p.per_kv = Divisor(p.kv_heads);
     p.per_part = Divisor(p.parts);
-    const int fill = p.fill ? 8 : 0;
-    p.fill = fill;
-    const dim3 grid(static_cast<uint32_t>(p.order.blocks() + fill));
+    p.fill = p.fill ? FILLERS : 0;
+    const dim3 grid(static_cast<uint32_t>(p.order.blocks() + p.fill));
     if (p.softcap > 0.0f)
         hipLaunchKernelGGL((attention_mass_kernel<D, FMT, KT, true>), grid, dim3(THREADS), 0, stream, p);
     else
@@ -227,24 +222,33 @@ int launch(MassParams p, int max_queries, int max_keys, hipStream_t stream) {
     return check_launch("mass_sum_kernel");
 }
 
+// Keys to a wave: 32, or 64 of 128 channels, for which every query fragment read from LDS feeds two products, where six
+// workgroups to a CU are left. With 32 and 64: 1 x 4000 tokens, 32 heads on 8: 91 and 113 us; 8 x 1000: 55 and 65; 8 x 4000:
+// 586 and 566; 1 x 16000: 1045 and 982. Heads of 64 channels are bound by the exponentials, and more waves hide more of the
+// rest (1 x 16000 tokens, 16 heads on 4: 407 and 474 us); 256 channels leave no registers for more.
 template <int FMT>
 int launch_dim(const MassParams& p, int max_queries, int max_keys, hipStream_t stream) {
-    if (p.head_dim == 64) return launch<64, FMT, 2>(p, max_queries, max_keys, stream);
-    if (p.head_dim == 128) return launch<128, FMT, 2>(p, max_queries, max_keys, stream);
-    return launch<256, FMT, 1>(p, max_queries, max_keys, stream);
+    if (p.head_dim == 64) return launch<64, FMT, 1>(p, max_queries, max_keys, stream);
+    if (p.head_dim == 256) return launch<256, FMT, 1>(p, max_queries, max_keys, stream);
+    constexpr int KEYS = WAVES * 64;
+    const int64_t by_longest = (static_cast<int64_t>(max_keys) + KEYS - 1) / KEYS * p.rows.sequences;
+    const int64_t by_rows = p.rows.k_rows / KEYS + p.rows.sequences;
+    const int64_t workgroups = (by_longest < by_rows ? by_longest : by_rows) * p.kv_heads * p.parts;
+    return workgroups >= 6 * 256 ? launch<128, FMT, 2>(p, max_queries, max_keys, stream)
+                                 : launch<128, FMT, 1>(p, max_queries, max_keys, stream);
 }
 
 }  // namespace
 
-size_t attention_mass_workspace(int max_queries, int64_t k_rows, int q_heads, int kv_heads) {
-    const int parts = parts_of(max_queries, q_heads / kv_heads);
+size_t attention_mass_workspace(int max_queries, int64_t k_rows, bool windowed, int q_heads, int kv_heads) {
+    const int parts = parts_of(max_queries, windowed, q_heads / kv_heads);
     return parts == 1 ? 0 : static_cast<size_t>(parts) * kv_heads * k_rows * sizeof(float);
 }
 
 int attention_mass(MassParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
                    hipStream_t stream) {
-    p.parts = parts_of(max_queries, p.groups);
-    const size_t need = attention_mass_workspace(max_queries, p.rows.k_rows, p.q_heads, p.kv_heads);
+    p.parts = parts_of(max_queries, p.window > 0, p.groups);
+    const size_t need = attention_mass_workspace(max_queries, p.rows.k_rows, p.window > 0, p.q_heads, p.kv_heads);
     if (need > 0 && (!workspace || workspace_bytes < need)) return fail("attention mass: the workspace is too small");
     p.partial = static_cast<float*>(workspace);
     return format == BF16 ? launch_dim<BF16>(p, max_queries, max_keys, stream)

@@ -112,7 +112,8 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
 size_t eco_attention_mass_workspace_size(int32_t max_queries, int64_t k_rows, int32_t window, int32_t q_heads,
                                          int32_t kv_heads) {
     if (max_queries < 0 || k_rows < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads) return 0;
-    return attention_mass_workspace(window > 0 && window < max_queries ? window : max_queries, k_rows, q_heads, kv_heads);
+    return attention_mass_workspace(window > 0 && window < max_queries ? window : max_queries, k_rows, window > 0, q_heads,
+                                    kv_heads);
 }
 
 int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t,

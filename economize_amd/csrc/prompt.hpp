@@ -26,6 +26,9 @@ struct Divisor {
     }
 };
 
+// Workgroups that look after the rows of no sequence, where a call asks for it.
+constexpr int FILLERS = 128;
+
 // Which (sequence, KV head) pair and which of its tiles a workgroup takes. The tiles of a pair read the same rows, so they
 // run close together: the pairs in `group` at a time, their longest tiles first. Workgroups go to the eight XCDs in turn,
 // each with an L2 of its own: with `pin` a pair stays on one.
@@ -36,15 +39,16 @@ struct WorkOrder {
     int64_t blocks() const { return static_cast<int64_t>(tiles) * (pin ? 8 * per_xcd() : pairs); }
 };
 
-// `tiles` per pair, whose rows read by all of them take `bytes`: as many pairs at a time as three quarters of an L2 hold.
+// `tiles` of `parts` workgroups each per pair, whose rows read by all of them take `bytes`: as many pairs at a time as three quarters of an L2 hold.
 // Pinned where that leaves the XCDs about the same work: with KV heads in eights each gets every sequence, otherwise many
 // sequences even out (6 sequences of different lengths with 4 KV heads, pinned: half of the CUs' time idle).
-inline WorkOrder work_order(int sequences, int kv_heads, int64_t tiles, int64_t bytes) {
+inline WorkOrder work_order(int sequences, int kv_heads, int64_t tiles, int parts, int64_t bytes) {
     const int64_t pairs = static_cast<int64_t>(sequences) * kv_heads;
-    if (tiles * pairs > (1 << 28)) tiles = (1 << 28) / pairs;
+    const int64_t most_tiles = (1 << 28) / (pairs * parts);
+    tiles = tiles < most_tiles ? tiles : most_tiles;
     WorkOrder o;
     o.pairs = static_cast<int>(pairs);
-    o.tiles = static_cast<int>(tiles < 1 ? 1 : tiles);
+    o.tiles = static_cast<int>(tiles < 1 ? 1 : tiles) * parts;
     o.pin = kv_heads % 8 == 0 || pairs >= 128;
     const int64_t fit = (3 << 20) / (bytes < 1 ? 1 : bytes);
     const int64_t most = o.pin ? o.per_xcd() : pairs;
@@ -66,7 +70,7 @@ struct PromptParams {
     int64_t so_t, so_h;
     float* lse;  // [Hq, sl_h] or null
     int64_t sl_h;
-    int fill;  // workgroups that give rows of no sequence out 0 and lse -inf (0: they are left as they are)
+    int fill;  // FILLERS workgroups give rows of no sequence out 0 and lse -inf (0: they are left as they are)
     int q_heads, kv_heads, groups, head_dim;
     Divisor per_group, per_kv, per_part;  // over the groups, the KV heads, the row tiles of a part
     WorkOrder order;  // (sequences of more row tiles than the launch holds loop over them)
@@ -88,7 +92,7 @@ struct MassParams {
     int64_t sl_h;
     float* mass;  // [Hkv, sm_h]
     int64_t sm_h;
-    int fill;    // workgroups that give keys of no sequence 0 (0: they are left as they are)
+    int fill;    // FILLERS workgroups give keys of no sequence 0 (0: they are left as they are)
     int window;  // only the last `window` queries of a sequence count
     int q_heads, kv_heads, groups, head_dim;
     Divisor per_kv, per_part;
@@ -100,6 +104,6 @@ struct MassParams {
 
 int attention_mass(MassParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
                    hipStream_t stream);
-size_t attention_mass_workspace(int max_queries, int64_t k_rows, int q_heads, int kv_heads);
+size_t attention_mass_workspace(int max_queries, int64_t k_rows, bool windowed, int q_heads, int kv_heads);
 
 }  // namespace eco

@@ -42,24 +42,19 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 31, half = lane >> 5;
-    const int fillers = p.fill, work = gridDim.x - fillers;
+    const int work = gridDim.x - p.fill;
     if (static_cast<int>(blockIdx.x) >= work) {  // the last workgroups: rows of no sequence
-        const int workers = fillers, me = blockIdx.x - work;
-        for (int g = 0; g <= p.rows.sequences; ++g) {
-            int64_t from = g == 0 ? 0 : p.rows.q_end[g - 1];
-            int64_t to = g == p.rows.sequences ? p.rows.q_rows : p.rows.q_begin[g];
-            from = from < 0 ? 0 : from;
-            to = to > p.rows.q_rows ? p.rows.q_rows : to;
-            if (to <= from) continue;
+        for_gaps(p.rows.q_begin, p.rows.q_end, p.rows.sequences, p.rows.q_rows, blockIdx.x - work,
+                 [&](int64_t from, int64_t to, int worker, int workers) {
             const int64_t chunks = (to - from) * p.q_heads * (D / 8);
-            for (int64_t c = static_cast<int64_t>(me) * THREADS + tid; c < chunks; c += static_cast<int64_t>(workers) * THREADS) {
+            for (int64_t c = static_cast<int64_t>(worker) * THREADS + tid; c < chunks; c += static_cast<int64_t>(workers) * THREADS) {
                 const int64_t row = c / (D / 8);
                 const int64_t t = from + row / p.q_heads;
                 const int h = static_cast<int>(row % p.q_heads);
                 *reinterpret_cast<uint4*>(p.out + t * p.so_t + h * p.so_h + (c % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
                 if (p.lse && c % (D / 8) == 0) p.lse[h * p.sl_h + t] = -INFINITY;
             }
-        }
+        });
         return;
     }
     int pair, slot;
@@ -449,12 +444,11 @@ int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
     constexpr int ROWS = WAVES * 32 * QT;
     const int64_t tiles = (static_cast<int64_t>(max_queries) * p.groups + ROWS - 1) / ROWS;
     const int64_t bytes = static_cast<int64_t>(max_keys) * D * 4;
-    p.order = work_order(p.rows.sequences, p.kv_heads, (tiles < 1 ? 1 : tiles) * p.parts, bytes);
-    p.order.tiles = p.order.tiles < p.parts ? p.parts : p.order.tiles / p.parts * p.parts;
+    p.order = work_order(p.rows.sequences, p.kv_heads, tiles, p.parts, bytes);
     p.per_group = Divisor(p.groups);
     p.per_kv = Divisor(p.kv_heads);
     p.per_part = Divisor(p.order.tiles / p.parts);
-    p.fill = p.fill ? 32 : 0;
+    p.fill = p.fill ? FILLERS : 0;
     const dim3 grid(static_cast<uint32_t>(p.order.blocks() + p.fill));
     if (p.softcap > 0.0f)
         hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, QT, WAVES, true>), grid, dim3(WAVES * 64), 0, stream, p);
@@ -462,7 +456,7 @@ int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
         hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, QT, WAVES, false>), grid, dim3(WAVES * 64), 0, stream, p);
     if (int rc = check_launch("prompt_attention_kernel")) return rc;
     if (p.parts == 1) return 0;
-    p.order = work_order(p.rows.sequences, p.kv_heads, tiles, bytes);
+    p.order = work_order(p.rows.sequences, p.kv_heads, tiles, 1, bytes);
     hipLaunchKernelGGL((prompt_join_kernel<D, FMT, ROWS>), dim3(static_cast<uint32_t>(p.order.blocks()), ROWS / JOINED),
                        dim3(256), 0, stream, p);
     return check_launch("prompt_join_kernel");

@@ -73,6 +73,22 @@ __device__ __forceinline__ bool work_of(const WorkOrder& o, int id, int& pair, i
     return pair < o.pairs;
 }
 
+// The rows of no sequence, by FILLERS workgroups, of which this is `me`: visit(from, to, worker, workers) for its share of
+// the gaps before, between and behind the sequences. (Gaps side by side: one after the other each costs a chain of two loads.)
+template <typename Visit>
+__device__ __forceinline__ void for_gaps(const int32_t* begin, const int32_t* end, int sequences, int64_t rows, int me, Visit visit) {
+    const int gaps = sequences + 1, at_once = gaps < 32 ? gaps : 32;
+    const int worker = me / at_once, workers = FILLERS / at_once;
+    if (worker >= workers) return;
+    for (int g = me - worker * at_once; g < gaps; g += at_once) {
+        int64_t from = g == 0 ? 0 : end[g - 1];
+        int64_t to = g == sequences ? rows : begin[g];
+        from = from < 0 ? 0 : from;
+        to = to > rows ? rows : to;
+        if (from < to) visit(from, to, worker, workers);
+    }
+}
+
 // A tile of 64 rows of D 16-bit channels in LDS, in chunks of 16 bytes. Keys are read as MFMA operands of 32 rows by 16
 // channels (ds_read_b128, lane l row l % 32), values transposed (ds_read_b64_tr_b16, 4 rows by 64 bytes for 32 lanes); the
 // two swizzles spread the rows of one such read over all 64 banks.
@@ -85,59 +101,6 @@ struct Tile {
     }
     static __device__ __forceinline__ int value_chunk(int row, int chunk) {
         return CHUNKS == 8 ? chunk ^ (((row >> 1) & 1) << 2) : chunk ^ ((row & 3) << 2);
-    }
-};
-
-// Rows [row0, row0 + 64) of a sequence's keys or values into registers: rows past its end read as zero (the buffer
-// resource ends with the sequence).
-template <int D, int THREADS>
-struct TileLoad {
-    static constexpr int N = 64 * (D / 8) / THREADS;
-    uint4 x[N];
-
-    __device__ __forceinline__ void load(const uint16_t* base, int64_t stride, int row0, int rows, int tid) {
-        const int left = rows - row0;
-        const int n = left < 64 ? left : 64;
-        const uint32_t bytes = n <= 0 ? 0u : static_cast<uint32_t>((n - 1) * stride * 2 + D * 2);
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint16_t*>(base + static_cast<int64_t>(row0) * stride), 0, bytes, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = tid + i * THREADS;
-            const uint32_t off = static_cast<uint32_t>(c / (D / 8)) * static_cast<uint32_t>(stride * 2) +
-                                 static_cast<uint32_t>(c % (D / 8)) * 16u;
-            x[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
-        }
-    }
-
-    // Infinities and NaN to 0; whether there was one.
-    template <int FMT>
-    __device__ __forceinline__ bool drop_non_finite() {
-        constexpr uint32_t LIMIT = FMT == BF16 ? 0x7F80u : 0x7C00u;
-        uint32_t big = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t m = max_magnitude8(x[i]);
-            big = m > big ? m : big;
-        }
-        if (big < LIMIT) return false;
-        auto clean = [](uint32_t w) {
-            return ((w & 0x7FFFu) >= LIMIT ? 0u : w & 0xFFFFu) | ((w >> 16 & 0x7FFFu) >= LIMIT ? 0u : w & 0xFFFF0000u);
-        };
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = make_uint4(clean(x[i].x), clean(x[i].y), clean(x[i].z), clean(x[i].w));
-        return true;
-    }
-
-    template <bool KEYS>
-    __device__ __forceinline__ void store(uint8_t* lds, int tid) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = tid + i * THREADS;
-            const int row = c / (D / 8), chunk = c % (D / 8);
-            const int to = KEYS ? Tile<D>::key_chunk(row, chunk) : Tile<D>::value_chunk(row, chunk);
-            *reinterpret_cast<uint4*>(lds + row * (D * 2) + to * 16) = x[i];
-        }
     }
 };
 
