@@ -11,6 +11,8 @@ namespace eco {
 
 namespace {
 
+constexpr int64_t MOST_ROWS = 0x7fff0000;  // (a tile past the last row is still a 32-bit index)
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check_shape(const char* what, int format, int q_heads, int kv_heads, int head_dim, float scale, float softcap) {
@@ -37,8 +39,18 @@ int check_packed(const char* what, const PackedRows& r) {
     const std::string w = what;
     if (!r.q_begin || !r.q_end || !r.k_begin || !r.k_end) return fail(w + ": null sequence bounds");
     if (r.sequences <= 0) return fail(w + ": need at least one sequence");
-    if (r.q_rows < 0 || r.k_rows < 0 || r.q_rows > 0x7fffffff || r.k_rows > 0x7fffffff)
-        return fail(w + ": rows must be from 0 to 2^31 - 1");
+    if (r.q_rows < 0 || r.k_rows < 0 || r.q_rows > MOST_ROWS || r.k_rows > MOST_ROWS)
+        return fail(w + ": rows must be from 0 to 2^31 - 2^16");
+    return 0;
+}
+
+// Outputs [rows, heads, D] of these strides hold no element twice.
+int check_apart(const char* what, int64_t rows, int64_t heads, int64_t s_row, int64_t s_head, int head_dim) {
+    const bool heads_within = s_head <= s_row;
+    const int64_t inner = heads_within ? s_head : s_row, outer = heads_within ? s_row : s_head;
+    const int64_t n = heads_within ? heads : rows, m = heads_within ? rows : heads;
+    if ((n > 1 && inner < head_dim) || (m > 1 && outer < (n > 1 ? (n - 1) * inner : 0) + head_dim))
+        return fail(std::string(what) + ": the outputs overlap each other");
     return 0;
 }
 
@@ -50,7 +62,8 @@ int check_cache(const char* what, const BudgetCache& c) {
     if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return fail(w + ": head dim must be 64, 128 or 256");
     if (c.recent < 1 || c.first < 0 || static_cast<int64_t>(c.recent) + c.first > c.slots)
         return fail(w + ": need recent >= 1, first >= 0 and recent + first <= slots");
-    if (static_cast<int64_t>(c.batch) * c.kv_heads > 0x3fffffff / c.slots)
+    if (static_cast<int64_t>(c.batch) * c.kv_heads > 65535) return fail(w + ": the cache has too many rows for one call");
+    if (c.slots > (1 << 25) || static_cast<int64_t>(c.batch) * c.kv_heads > 0x3fffffff / c.slots)
         return fail(w + ": the cache has too many slots for one call");
     return 0;
 }
@@ -88,10 +101,11 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
     if (int rc = check_rows("prompt attention: keys", k, {sk_t, sk_h})) return rc;
     if (int rc = check_rows("prompt attention: values", v, {sv_t, sv_h})) return rc;
     if (int rc = check_rows("prompt attention: outputs", out, {so_t, so_h})) return rc;
+    if (int rc = check_apart(what, q_rows, q_heads, so_t, so_h, head_dim)) return rc;
     if (lse && sl_h < q_rows) return fail("prompt attention: lse rows are shorter than the queries");
     if (max_queries < 0 || max_keys < 0) return fail("prompt attention: sizes must not be negative");
     if (static_cast<int64_t>(sequences) * kv_heads > 65535) return fail("prompt attention: too many sequences");
-    if (q_rows > 0x7fff0000 / (q_heads / kv_heads)) return fail("prompt attention: too many queries for one call");
+    if (q_rows > MOST_ROWS / (q_heads / kv_heads)) return fail("prompt attention: too many queries for one call");
     PromptParams p{};
     p.q = static_cast<const uint16_t*>(q);
     p.k = static_cast<const uint16_t*>(k);
@@ -132,7 +146,7 @@ int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h
     if (int rc = check_rows("attention mass: keys", k, {sk_t, sk_h})) return rc;
     if (sl_h < q_rows) return fail("attention mass: lse rows are shorter than the queries");
     if (sm_h < k_rows) return fail("attention mass: mass rows are shorter than the keys");
-    if (q_rows > 0x7fff0000 / (q_heads / kv_heads)) return fail("attention mass: too many queries for one call");
+    if (q_rows > MOST_ROWS / (q_heads / kv_heads)) return fail("attention mass: too many queries for one call");
     if (window < 0 || max_queries < 0 || max_keys < 0) return fail("attention mass: sizes must not be negative");
     if (static_cast<int64_t>(sequences) * kv_heads > 65535) return fail("attention mass: too many sequences");
     MassParams p{};
@@ -162,8 +176,25 @@ int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, i
     if (int rc = check_cache(what, p.cache)) return rc;
     if (int rc = check_rows("prompt eviction: keys", k, {sk_t, sk_h})) return rc;
     if (int rc = check_rows("prompt eviction: values", v, {sv_t, sv_h})) return rc;
-    if (rows < 0 || rows > 0x7fffffff || max_tokens < 0) return fail("prompt eviction: rows must be from 0 to 2^31 - 1");
+    if (rows < 0 || rows > MOST_ROWS || max_tokens < 0) return fail("prompt eviction: rows must be from 0 to 2^31 - 2^16");
     if (sm_h < rows) return fail("prompt eviction: mass rows are shorter than the keys");
+    // (tokens are copied in any order: a slot may be written before the token it held is read)
+    const int64_t cells = static_cast<int64_t>(batch) * kv_heads * slots;
+    struct Span {
+        uintptr_t at;
+        int64_t bytes;
+    };
+    const Span to[] = {{reinterpret_cast<uintptr_t>(keys), cells * head_dim * 2},
+                       {reinterpret_cast<uintptr_t>(values), cells * head_dim * 2},
+                       {reinterpret_cast<uintptr_t>(score), cells * 4},
+                       {reinterpret_cast<uintptr_t>(position), cells * 4}};
+    const Span from[] = {{reinterpret_cast<uintptr_t>(k), ((rows - 1) * sk_t + (kv_heads - 1) * sk_h + head_dim) * 2},
+                         {reinterpret_cast<uintptr_t>(v), ((rows - 1) * sv_t + (kv_heads - 1) * sv_h + head_dim) * 2},
+                         {reinterpret_cast<uintptr_t>(mass), ((kv_heads - 1) * sm_h + rows) * 4}};
+    for (const Span& a : from)
+        for (const Span& b : to)
+            if (rows > 0 && a.at < b.at + b.bytes && b.at < a.at + a.bytes)
+                return fail("prompt eviction: the prompt must be in memory apart from the cache's");
     p.k = static_cast<const uint16_t*>(k);
     p.v = static_cast<const uint16_t*>(v);
     p.sk_t = sk_t, p.sk_h = sk_h, p.sv_t = sv_t, p.sv_h = sv_h;
@@ -198,6 +229,7 @@ int eco_heavy_hitter_decode(const void* q, int32_t format, int64_t sq_b, int64_t
     if (int rc = check_rows("heavy-hitter decode: keys", k, {sk_b, sk_h})) return rc;
     if (int rc = check_rows("heavy-hitter decode: values", v, {sv_b, sv_h})) return rc;
     if (int rc = check_rows("heavy-hitter decode: outputs", out, {so_b, so_h})) return rc;
+    if (int rc = check_apart(what, batch, q_heads, so_b, so_h, head_dim)) return rc;
     p.q = static_cast<const uint16_t*>(q);
     p.sq_b = sq_b, p.sq_h = sq_h;
     p.k = static_cast<const uint16_t*>(k);

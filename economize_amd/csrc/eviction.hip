@@ -171,33 +171,34 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictParams p) {
     }
 }
 
-// The kept tokens' keys and values: one 16-byte chunk per thread.
+// The kept tokens' keys and values: one 16-byte chunk per thread, where the launch holds the longest row.
 __global__ __launch_bounds__(256) void evict_copy_kernel(EvictParams p) {
     const BudgetCache& c = p.cache;
     const int chunks = c.head_dim / 8;
     const int bh = blockIdx.y, b = bh / c.kv_heads, h = bh % c.kv_heads;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int slot = static_cast<int>(at / chunks), chunk = static_cast<int>(at % chunks);
-    if (slot >= c.count[bh] || slot >= c.slots) return;
+    const int64_t kept = static_cast<int64_t>(c.count[bh]) * chunks;
     int64_t from = p.begin[b];
     from = from < 0 ? 0 : from;
-    int64_t row = from + c.position[static_cast<int64_t>(bh) * c.slots + slot];
-    const int64_t to = (static_cast<int64_t>(bh) * c.slots + slot) * c.head_dim + chunk * 8;
-    *reinterpret_cast<uint4*>(c.keys + to) = *reinterpret_cast<const uint4*>(p.k + row * p.sk_t + h * p.sk_h + chunk * 8);
-    *reinterpret_cast<uint4*>(c.values + to) =
-        *reinterpret_cast<const uint4*>(p.v + row * p.sv_t + h * p.sv_h + chunk * 8);
+    for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < kept; at += static_cast<int64_t>(gridDim.x) * 256) {
+        const int slot = static_cast<int>(at / chunks), chunk = static_cast<int>(at % chunks);
+        const int64_t row = from + c.position[static_cast<int64_t>(bh) * c.slots + slot];
+        const int64_t to = (static_cast<int64_t>(bh) * c.slots + slot) * c.head_dim + chunk * 8;
+        *reinterpret_cast<uint4*>(c.keys + to) =
+            *reinterpret_cast<const uint4*>(p.k + row * p.sk_t + h * p.sk_h + chunk * 8);
+        *reinterpret_cast<uint4*>(c.values + to) =
+            *reinterpret_cast<const uint4*>(p.v + row * p.sv_t + h * p.sv_h + chunk * 8);
+    }
 }
 
 }  // namespace
 
 int evict_prompt(const EvictParams& p, int max_tokens, hipStream_t stream) {
-    (void)max_tokens;
     const BudgetCache& c = p.cache;
     hipLaunchKernelGGL(evict_select_kernel, dim3(c.batch * c.kv_heads), dim3(THREADS), 0, stream, p);
     if (int rc = check_launch("evict_select_kernel")) return rc;
-    const int64_t chunks = static_cast<int64_t>(c.slots) * (c.head_dim / 8);
-    hipLaunchKernelGGL(evict_copy_kernel, dim3(static_cast<uint32_t>((chunks + 255) / 256), c.batch * c.kv_heads),
-                       dim3(256), 0, stream, p);
+    const int64_t chunks = static_cast<int64_t>(max_tokens < c.slots ? max_tokens : c.slots) * (c.head_dim / 8);
+    const uint32_t blocks = static_cast<uint32_t>(chunks > 256 ? (chunks + 255) / 256 : 1);
+    hipLaunchKernelGGL(evict_copy_kernel, dim3(blocks, c.batch * c.kv_heads), dim3(256), 0, stream, p);
     return check_launch("evict_copy_kernel");
 }
 

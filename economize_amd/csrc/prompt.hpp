@@ -44,7 +44,7 @@ struct WorkOrder {
 // sequences even out (6 sequences of different lengths with 4 KV heads, pinned: half of the CUs' time idle).
 inline WorkOrder work_order(int sequences, int kv_heads, int64_t tiles, int parts, int64_t bytes) {
     const int64_t pairs = static_cast<int64_t>(sequences) * kv_heads;
-    const int64_t most_tiles = (1 << 28) / (pairs * parts);
+    const int64_t most_tiles = (1 << 23) / (pairs * parts);
     tiles = tiles < most_tiles ? tiles : most_tiles;
     WorkOrder o;
     o.pairs = static_cast<int>(pairs);

@@ -3,9 +3,9 @@
 // With x_ij = scale q_i . k_j (soft-capped or not), query i gives o_i = sum_j exp(x_ij - lse_i) v_j over the keys it sees,
 // lse_i = log(sum_j exp(x_ij) + exp(sink)). One pass over the keys with a running maximum and sum (both fp32).
 //
-// A workgroup holds 128 QT rows of one (sequence, KV head): row r is query r / G of head r % G of the group, so the G
+// A workgroup holds 128 rows of one (sequence, KV head): row r is query r / G of head r % G of the group, so the G
 // heads of a group share every K/V tile and a tile's rows span few queries (little of the causal diagonal is wasted).
-// A wave holds 32 QT rows as columns: S^T = K Q^T puts one query in each lane (l % 32) with 16 of 32 keys in its
+// A wave holds 32 rows as columns: S^T = K Q^T puts one query in each lane (l % 32) with 16 of 32 keys in its
 // registers, so the softmax needs one exchange with lane l ^ 32 and P^T is already the second product's operand: its eight
 // keys per lane are {4 h .. 4 h + 3, 8 + 4 h ..} of 16 (h = l / 32), the order the transposed value reads deliver.
 // O^T keeps the query in the lane, so rescaling is one multiplier per lane.
@@ -15,6 +15,9 @@
 namespace eco {
 
 namespace {
+
+constexpr int WAVES = 4, THREADS = WAVES * 64;
+constexpr int ROWS = WAVES * 32;  // rows of a tile
 
 constexpr float NEVER = -1e30f;  // running maximum before the first key (log2 units)
 
@@ -30,13 +33,11 @@ __device__ __forceinline__ int part_begin(int key_tiles, int part, int parts) {
     return static_cast<int>(static_cast<int64_t>(key_tiles) * part / parts);
 }
 
-template <int D, int FMT, int QT, int WAVES, bool CAP>
-__global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) void prompt_attention_kernel(PromptParams p) {
-    constexpr int THREADS = WAVES * 64;
+template <int D, int FMT, bool CAP>
+__global__ __launch_bounds__(THREADS, D == 256 ? 1 : D == 128 ? 2 : 3) void prompt_attention_kernel(PromptParams p) {
     typedef Tile<D> T;
     constexpr int KS = D / 16;  // 16-channel steps of the first product
     constexpr int DT = D / 32;  // 32-channel blocks of the output
-    constexpr int ROWS = WAVES * 32 * QT;
     __shared__ __align__(256) uint8_t lds[4][T::BYTES];
     __shared__ int unseen;  // an infinity or a NaN was taken out of the values of a tile that not every row sees
 
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
 
     for (int t = first; t < tiles; t += stride) {
         const int low_row = (tiles - 1 - t) * ROWS;  // the longest rows first
-        const int row0 = low_row + wave * 32 * QT;
+        const int row0 = low_row + wave * 32;
         const int last = over_groups(low_row + ROWS - 1 < total ? low_row + ROWS - 1 : total - 1) + offset;
         const int full = over_groups(low_row) + offset;  // every row of the tile sees keys <= full, some keys <= last
         const int wave_full = over_groups(row0 < total ? row0 : total - 1) + offset;
@@ -99,112 +100,83 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
             values(from);
             if (key_tiles > from + 1) keys(from + 1);
         }
-        int qi[QT], head[QT], limit[QT];
-        uint4 qf[QT][KS];
+        const bool live = row0 + col < total;  // the lane's row
+        const int row_at = live ? row0 + col : total - 1;
+        const int qi = over_groups(row_at), head = row_at - qi * p.groups;
+        const int limit = live ? qi + offset : -1;
+        uint4 qf[KS];
+        const uint16_t* qp = p.q + (seq.q0 + qi) * p.sq_t + (kvh * p.groups + head) * p.sq_h + half * 8;
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            const int r = row0 + 32 * u + col;
-            const int rr = r < total ? r : total - 1;
-            qi[u] = over_groups(rr);
-            head[u] = rr - qi[u] * p.groups;
-            limit[u] = r < total ? qi[u] + offset : -1;
-            const uint16_t* qp = p.q + (seq.q0 + qi[u]) * p.sq_t + (kvh * p.groups + head[u]) * p.sq_h + half * 8;
-#pragma unroll
-            for (int i = 0; i < KS; ++i) qf[u][i] = *reinterpret_cast<const uint4*>(qp + 16 * i);
-        }
+        for (int i = 0; i < KS; ++i) qf[i] = *reinterpret_cast<const uint4*>(qp + 16 * i);
 
-        f32x16 acc[QT][DT];
-        float m[QT], l0[QT], l1[QT];
+        f32x16 acc[DT];
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) acc[u][d] = f32x16{};
-            m[u] = NEVER;
-            l0[u] = l1[u] = 0.0f;
-        }
-        f32x16 sa[QT][2], sb[QT][2];
+        for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+        float m = NEVER, l0 = 0.0f, l1 = 0.0f;
+        f32x16 sa[2], sb[2];
 
         // S^T of tile j
-        auto scores = [&](int j, f32x16 (&x)[QT][2]) {
+        auto scores = [&](int j, f32x16 (&x)[2]) {
             uint32_t at = lds_address(lds[j & 1]) + kplace;
             asm volatile("" : "+v"(at));  // (computed here: held for every channel step and buffer it would not fit)
 #pragma unroll
-            for (int u = 0; u < QT; ++u)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) x[u][b] = f32x16{};
+            for (int b = 0; b < 2; ++b) x[b] = f32x16{};
 #pragma unroll
             for (int i = 0; i < KS; ++i)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const uint4 kf = lds_read16((at ^ (32 * i)) + 32 * b * (D * 2));
-#pragma unroll
-                    for (int u = 0; u < QT; ++u) x[u][b] = mfma32<FMT>(kf, qf[u][i], x[u][b]);
+                    x[b] = mfma32<FMT>(kf, qf[i], x[b]);
                 }
         };
-        auto hide = [&](int j, f32x16 (&x)[QT][2]) {  // soft cap, and what the lane's query does not see
+        auto hide = [&](int j, f32x16 (&x)[2]) {  // soft cap, and what the lane's query does not see
             if constexpr (CAP) {
-#pragma unroll
-                for (int u = 0; u < QT; ++u)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            x[u][b][i] = soft_cap_log2(x[u][b][i] * p.scale, p.softcap, 1.0f / p.softcap);
-            }
-            if (64 * j + 63 > wave_full) {
-#pragma unroll
-                for (int u = 0; u < QT; ++u) {
-                    const int seen = limit[u] - 64 * j - 4 * half;
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (32 * b + 8 * (i >> 2) + (i & 3) > seen) x[u][b][i] = -INFINITY;
-                }
-            }
-        };
-        // The maximum moves only when it grows by more than 2^8: weights stay below 2^8.
-        auto raise = [&](const f32x16 (&x)[QT][2]) {
-            float mn[QT];
-            bool up = false;
-#pragma unroll
-            for (int u = 0; u < QT; ++u) {
-                float mx[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx[i] = max_nan(x[u][0][i], x[u][1][i]);
-#pragma unroll
-                for (int i = 4; i < 16; ++i) mx[i & 3] = max_nan(max_nan(mx[i & 3], x[u][0][i]), x[u][1][i]);
-                mn[u] = swap_max(max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]))) * cc;
-                up |= mn[u] > m[u] + 8.0f;
-            }
-            if (__ballot(up)) {
-#pragma unroll
-                for (int u = 0; u < QT; ++u) {
-                    const float to = mn[u] > m[u] ? mn[u] : m[u];
-                    const float a = __builtin_amdgcn_exp2f(m[u] - to);
-                    m[u] = to;
-                    l0[u] *= a;
-                    l1[u] *= a;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) acc[u][d] *= a;
-                }
-            }
-        };
-        auto weights = [&](const f32x16 (&x)[QT][2], uint32_t (&pf)[QT][16]) {
-#pragma unroll
-            for (int u = 0; u < QT; ++u)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][b][i], cc, -m[u]));
-                        const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][b][i + 1], cc, -m[u]));
-                        l0[u] += y;
-                        l1[u] += z;
-                        pf[u][8 * b + (i >> 1)] = pack_pair<FMT>(y, z);
-                    }
+                    for (int i = 0; i < 16; ++i)
+                        x[b][i] = soft_cap_log2(x[b][i] * p.scale, p.softcap, 1.0f / p.softcap);
+            }
+            if (64 * j + 63 > wave_full) {
+                const int seen = limit - 64 * j - 4 * half;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (32 * b + 8 * (i >> 2) + (i & 3) > seen) x[b][i] = -INFINITY;
+            }
         };
-        auto products = [&](int j, const uint32_t (&pf)[QT][16]) {
+        // The maximum moves only when it grows by more than 2^8: weights stay below 2^8.
+        auto raise = [&](const f32x16 (&x)[2]) {
+            float mx[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i] = max_nan(x[0][i], x[1][i]);
+#pragma unroll
+            for (int i = 4; i < 16; ++i) mx[i & 3] = max_nan(max_nan(mx[i & 3], x[0][i]), x[1][i]);
+            const float mn = swap_max(max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]))) * cc;
+            if (__ballot(mn > m + 8.0f)) {
+                const float to = mn > m ? mn : m;
+                const float a = __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l0 *= a;
+                l1 *= a;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[d] *= a;
+            }
+        };
+        auto weights = [&](const f32x16 (&x)[2], uint32_t (&pf)[16]) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i], cc, -m));
+                    const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i + 1], cc, -m));
+                    l0 += y;
+                    l1 += z;
+                    pf[8 * b + (i >> 1)] = pack_pair<FMT>(y, z);
+                }
+        };
+        auto products = [&](int j, const uint32_t (&pf)[16]) {
             uint32_t at = lds_address(lds[2 + (j & 1)]) + vplace;
             asm volatile("" : "+v"(at));
 #pragma unroll
@@ -215,10 +187,7 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
 #pragma unroll
                     for (int e = 0; e < 2; ++e) w[e] = lds_read_transposed((at ^ (64 * d)) + (16 * b + 8 * e) * (D * 2));
                     const uint4 vf = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
-#pragma unroll
-                    for (int u = 0; u < QT; ++u)
-                        acc[u][d] = mfma32<FMT>(vf, make_uint4(pf[u][4 * b], pf[u][4 * b + 1], pf[u][4 * b + 2],
-                                                               pf[u][4 * b + 3]), acc[u][d]);
+                    acc[d] = mfma32<FMT>(vf, make_uint4(pf[4 * b], pf[4 * b + 1], pf[4 * b + 2], pf[4 * b + 3]), acc[d]);
                 }
         };
         // Tile j's values have arrived and are about to be used. A weight of 0 times an infinity or a NaN would be a NaN: in
@@ -236,24 +205,21 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
             clean(j);
         };
         // One tile: its weights while the next tile's scores are computed, then its products.
-        auto step = [&](int j, f32x16 (&cur)[QT][2], f32x16 (&nxt)[QT][2]) {
+        auto step = [&](int j, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
             arrive(j);
-            uint32_t pf[QT][16];
+            uint32_t pf[16];
             scores(j + 1, nxt);
             weights(cur, pf);
 #pragma unroll
             for (int i = 0; i < 2 * KS; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, QT, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, (112 * QT + 2 * KS - 1) / (2 * KS), 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, (112 + 2 * KS - 1) / (2 * KS), 0);
             }
             // (the weights belong here: left to itself the compiler moves them behind the masks)
-#pragma unroll
-            for (int u = 0; u < QT; ++u)
-                asm volatile("" : "+v"(pf[u][0]), "+v"(pf[u][1]), "+v"(pf[u][2]), "+v"(pf[u][3]), "+v"(pf[u][4]),
-                             "+v"(pf[u][5]), "+v"(pf[u][6]), "+v"(pf[u][7]), "+v"(pf[u][8]), "+v"(pf[u][9]),
-                             "+v"(pf[u][10]), "+v"(pf[u][11]), "+v"(pf[u][12]), "+v"(pf[u][13]), "+v"(pf[u][14]),
-                             "+v"(pf[u][15]), "+v"(l0[u]), "+v"(l1[u]));
+            asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pf[2]), "+v"(pf[3]), "+v"(pf[4]), "+v"(pf[5]), "+v"(pf[6]),
+                         "+v"(pf[7]), "+v"(pf[8]), "+v"(pf[9]), "+v"(pf[10]), "+v"(pf[11]), "+v"(pf[12]), "+v"(pf[13]),
+                         "+v"(pf[14]), "+v"(pf[15]), "+v"(l0), "+v"(l1));
             hide(j + 1, nxt);
             products(j, pf);
             raise(nxt);
@@ -272,14 +238,11 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
         }
         if (j + 1 < key_tiles) {
             step(j++, sa, sb);
-#pragma unroll
-            for (int u = 0; u < QT; ++u) {
-                sa[u][0] = sb[u][0];
-                sa[u][1] = sb[u][1];
-            }
+            sa[0] = sb[0];
+            sa[1] = sb[1];
         }
         if (j < key_tiles) {
-            uint32_t pf[QT][16];
+            uint32_t pf[16];
             arrive(j);
             weights(sa, pf);
             products(j, pf);
@@ -290,77 +253,72 @@ __global__ __launch_bounds__(WAVES * 64, (D * QT >= 256 || WAVES == 8 ? 1 : 2)) 
             for (int key = unseen_from > 64 * from ? unseen_from : 64 * from; key <= upto; ++key) {
                 const uint16_t* vp = vbase + key * p.sv_t + 4 * half;
 #pragma unroll
-                for (int u = 0; u < QT; ++u)
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint32_t x = vp[32 * d + 8 * (i >> 2) + (i & 3)];
-                            float v, none;
-                            unpack_pair<FMT>(x, v, none);
-                            if (key <= limit[u] && (x & 0x7FFFu) >= (FMT == BF16 ? 0x7F80u : 0x7C00u)) acc[u][d][i] += v;
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t x = vp[32 * d + 8 * (i >> 2) + (i & 3)];
+                        float v, none;
+                        unpack_pair<FMT>(x, v, none);
+                        if (key <= limit && (x & 0x7FFFu) >= (FMT == BF16 ? 0x7F80u : 0x7C00u)) acc[d][i] += v;
+                    }
             }
         }
         // The wave's 32 rows through LDS (the tiles are used up), so that whole rows are written
         constexpr int PITCH = D * 2 + 16;
         static_assert(WAVES * 32 * PITCH <= sizeof(lds), "the rows fit the tiles");
         uint8_t* mine = &lds[0][0] + wave * 32 * PITCH;
+        const float sum = swap_sum(l0 + l1);
+        const int h = kvh * p.groups + head;
+        const int64_t token = seq.q0 + qi;
+        if (parts > 1) {  // the part's maximum, sum and products, joined with the others by prompt_join_kernel
+            if (row0 + col < total) {
+                const int64_t row = (static_cast<int64_t>(part) * p.rows.q_rows + token) * p.q_heads + h;
+                if (half == 0) *reinterpret_cast<float2*>(p.part_stats + 2 * row) = make_float2(m, sum);
+                float* to = p.part_out + row * D + 4 * half;
 #pragma unroll
-        for (int u = 0; u < QT; ++u) {
-            const float sum = swap_sum(l0[u] + l1[u]);
-            const int h = kvh * p.groups + head[u];
-            const int64_t token = seq.q0 + qi[u];
-            if (parts > 1) {  // the part's maximum, sum and products, joined with the others by prompt_join_kernel
-                if (row0 + 32 * u + col < total) {
-                    const int64_t row = (static_cast<int64_t>(part) * p.rows.q_rows + token) * p.q_heads + h;
-                    if (half == 0) *reinterpret_cast<float2*>(p.part_stats + 2 * row) = make_float2(m[u], sum);
-                    float* to = p.part_out + row * D + 4 * half;
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            *reinterpret_cast<float4*>(to + 32 * d + 8 * i) =
-                                make_float4(acc[u][d][4 * i], acc[u][d][4 * i + 1], acc[u][d][4 * i + 2], acc[u][d][4 * i + 3]);
-                }
-                continue;
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float4*>(to + 32 * d + 8 * i) =
+                            make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
             }
-            float scale = 1.0f, den = sum, top = m[u];
-            if (p.sinks) {
-                const float sink = p.sinks[h] * kLog2e;
-                top = sink > m[u] ? sink : m[u];
-                scale = __builtin_amdgcn_exp2f(m[u] - top);
-                den = sum * scale + __builtin_amdgcn_exp2f(sink - top);
-            }
-            const float inv = den == 0.0f ? 0.0f : scale / den;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<uint2*>(mine + col * PITCH + (32 * d + 8 * i + 4 * half) * 2) =
-                        make_uint2(pack_pair<FMT>(acc[u][d][4 * i] * inv, acc[u][d][4 * i + 1] * inv),
-                                   pack_pair<FMT>(acc[u][d][4 * i + 2] * inv, acc[u][d][4 * i + 3] * inv));
-            if (p.lse && half == 0 && row0 + 32 * u + col < total)
-                p.lse[h * p.sl_h + token] = (top + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int i = 0; i < 32 * T::CHUNKS / 64; ++i) {
-                const int row = (lane + 64 * i) / T::CHUNKS, chunk = (lane + 64 * i) % T::CHUNKS;
-                const int r = row0 + 32 * u + row;
-                if (r >= total) continue;
-                const int q = over_groups(r);
-                *reinterpret_cast<uint4*>(p.out + (seq.q0 + q) * p.so_t + (kvh * p.groups + r - q * p.groups) * p.so_h +
-                                          chunk * 8) = *reinterpret_cast<const uint4*>(mine + row * PITCH + chunk * 16);
-            }
-            __builtin_amdgcn_wave_barrier();
+            continue;
         }
+        float scale = 1.0f, den = sum, top = m;
+        if (p.sinks) {
+            const float sink = p.sinks[h] * kLog2e;
+            top = sink > m ? sink : m;
+            scale = __builtin_amdgcn_exp2f(m - top);
+            den = sum * scale + __builtin_amdgcn_exp2f(sink - top);
+        }
+        const float inv = den == 0.0f ? 0.0f : scale / den;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint2*>(mine + col * PITCH + (32 * d + 8 * i + 4 * half) * 2) =
+                    make_uint2(pack_pair<FMT>(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv),
+                               pack_pair<FMT>(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv));
+        if (p.lse && half == 0 && row0 + col < total)
+            p.lse[h * p.sl_h + token] = (top + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 32 * T::CHUNKS / 64; ++i) {
+            const int row = (lane + 64 * i) / T::CHUNKS, chunk = (lane + 64 * i) % T::CHUNKS;
+            const int r = row0 + row;
+            if (r >= total) continue;
+            const int q = over_groups(r);
+            *reinterpret_cast<uint4*>(p.out + (seq.q0 + q) * p.so_t + (kvh * p.groups + r - q * p.groups) * p.so_h +
+                                      chunk * 8) = *reinterpret_cast<const uint4*>(mine + row * PITCH + chunk * 16);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
 // The parts of the rows whose keys were cut: four channels to a lane, JOINED rows of a row tile to a workgroup.
 constexpr int JOINED = 32;
 
-template <int D, int FMT, int ROWS>
+template <int D, int FMT>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
     int pair, first;
     if (!work_of(p.order, blockIdx.x, pair, first)) return;
@@ -422,26 +380,30 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptParams p) {
     }
 }
 
+size_t part_bytes(int parts, int64_t q_rows, int q_heads, int floats) {
+    return static_cast<size_t>(parts) * q_rows * q_heads * floats * sizeof(float);
+}
+
+// The parts' workspace has a place for every row, also where a few rows of a large buffer are sequences.
+constexpr int64_t MOST_PART_BYTES = 1 << 29;
+
 // Where there are too few row tiles for the GPU (six to a CU: prompt chunks of 6 sequences take 147 us at four, 142 at six,
 // 164 at sixteen), their keys are cut into up to so many parts.
-int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads) {
-    constexpr int ROWS = 128;
+int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads, int head_dim) {
+    if (q_rows == 0) return 1;
     const int64_t groups = q_heads / kv_heads;
     const int64_t by_longest = (max_queries * groups + ROWS - 1) / ROWS * sequences;
     const int64_t by_rows = q_rows * groups / ROWS + sequences;
     const int64_t row_tiles = (by_longest < by_rows ? by_longest : by_rows) * kv_heads;
-    const int64_t most = static_cast<int64_t>(max_keys) / (64 * MIN_PART);
+    int64_t most = static_cast<int64_t>(max_keys) / (64 * MIN_PART);
+    const int64_t fit = MOST_PART_BYTES / static_cast<int64_t>(part_bytes(1, q_rows, q_heads, head_dim + 2));
+    most = most < fit ? most : fit;
     const int64_t parts = row_tiles > 0 ? (1536 + row_tiles - 1) / row_tiles : 1;
     return static_cast<int>(parts < 1 || most < 1 ? 1 : parts < most ? parts : most);
 }
 
-size_t part_bytes(int parts, int64_t q_rows, int q_heads, int floats) {
-    return parts == 1 ? 0 : static_cast<size_t>(parts) * q_rows * q_heads * floats * sizeof(float);
-}
-
-template <int D, int FMT, int QT, int WAVES>
+template <int D, int FMT>
 int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
-    constexpr int ROWS = WAVES * 32 * QT;
     const int64_t tiles = (static_cast<int64_t>(max_queries) * p.groups + ROWS - 1) / ROWS;
     const int64_t bytes = static_cast<int64_t>(max_keys) * D * 4;
     p.order = work_order(p.rows.sequences, p.kv_heads, tiles, p.parts, bytes);
@@ -451,34 +413,35 @@ int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
     p.fill = p.fill ? FILLERS : 0;
     const dim3 grid(static_cast<uint32_t>(p.order.blocks() + p.fill));
     if (p.softcap > 0.0f)
-        hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, QT, WAVES, true>), grid, dim3(WAVES * 64), 0, stream, p);
+        hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, true>), grid, dim3(THREADS), 0, stream, p);
     else
-        hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, QT, WAVES, false>), grid, dim3(WAVES * 64), 0, stream, p);
+        hipLaunchKernelGGL((prompt_attention_kernel<D, FMT, false>), grid, dim3(THREADS), 0, stream, p);
     if (int rc = check_launch("prompt_attention_kernel")) return rc;
     if (p.parts == 1) return 0;
     p.order = work_order(p.rows.sequences, p.kv_heads, tiles, 1, bytes);
-    hipLaunchKernelGGL((prompt_join_kernel<D, FMT, ROWS>), dim3(static_cast<uint32_t>(p.order.blocks()), ROWS / JOINED),
+    hipLaunchKernelGGL((prompt_join_kernel<D, FMT>), dim3(static_cast<uint32_t>(p.order.blocks()), ROWS / JOINED),
                        dim3(256), 0, stream, p);
     return check_launch("prompt_join_kernel");
 }
 
 template <int FMT>
 int launch_dim(const PromptParams& p, int max_queries, int max_keys, hipStream_t stream) {
-    if (p.head_dim == 64) return launch<64, FMT, 1, 4>(p, max_queries, max_keys, stream);
-    if (p.head_dim == 128) return launch<128, FMT, 1, 4>(p, max_queries, max_keys, stream);
-    return launch<256, FMT, 1, 4>(p, max_queries, max_keys, stream);
+    if (p.head_dim == 64) return launch<64, FMT>(p, max_queries, max_keys, stream);
+    if (p.head_dim == 128) return launch<128, FMT>(p, max_queries, max_keys, stream);
+    return launch<256, FMT>(p, max_queries, max_keys, stream);
 }
 
 }  // namespace
 
 size_t prompt_attention_workspace(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads,
                                   int head_dim) {
-    return part_bytes(most_parts(sequences, q_rows, max_queries, max_keys, q_heads, kv_heads), q_rows, q_heads, head_dim + 2);
+    const int parts = most_parts(sequences, q_rows, max_queries, max_keys, q_heads, kv_heads, head_dim);
+    return parts == 1 ? 0 : part_bytes(parts, q_rows, q_heads, head_dim + 2);
 }
 
 int prompt_attention(PromptParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
                      hipStream_t stream) {
-    p.parts = most_parts(p.rows.sequences, p.rows.q_rows, max_queries, max_keys, p.q_heads, p.kv_heads);
+    p.parts = most_parts(p.rows.sequences, p.rows.q_rows, max_queries, max_keys, p.q_heads, p.kv_heads, p.head_dim);
     if (p.parts > 1 && (!workspace || workspace_bytes < part_bytes(p.parts, p.rows.q_rows, p.q_heads, p.head_dim + 2)))
         return fail("prompt attention: the workspace is too small");
     p.part_out = static_cast<float*>(workspace);

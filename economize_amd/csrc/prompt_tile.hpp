@@ -130,7 +130,8 @@ __device__ __forceinline__ uint2 lds_read_transposed(uint32_t at) {
 
 // Copies of 64-row tiles straight into LDS (buffer_load_dwordx4 ... lds: 64 lanes' 16 bytes in a row from the address in
 // M0), by a workgroup of THREADS. A lane's place in LDS is fixed, so it fetches the chunk the swizzle puts there. Rows past the
-// sequence's end are outside the buffer resource. The copies of a tile complete at the workgroup's next tile_barrier.
+// sequence's end are outside the buffer resource (the whole offset is the lane's: the scalar one is no part of the check).
+// The copies of a tile complete at the workgroup's next tile_barrier.
 template <int D, int THREADS>
 struct TileCopy {
     static constexpr int CHUNKS = D / 8, N = 64 * CHUNKS / THREADS, ROWS = THREADS / CHUNKS;  // rows per instruction
@@ -163,9 +164,10 @@ struct TileCopy {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + i * (THREADS * 16u));
-            const uint32_t skip = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(i * ROWS) * static_cast<uint32_t>(stride * 2));
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                         :: "s"(m0), "v"(from[i % KINDS]), "s"(rsrc), "s"(skip) : "memory");
+            uint32_t skip = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(i * ROWS) * static_cast<uint32_t>(stride * 2));
+            asm volatile("" : "+s"(skip));  // (added here: the sums held over the loop cost a wave of every SIMD)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :: "s"(m0), "v"(from[i % KINDS] + skip), "s"(rsrc) : "memory");
         }
     }
 };

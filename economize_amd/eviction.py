@@ -120,7 +120,7 @@ def evict_prompt(cache: HeavyHitterCache, key: torch.Tensor, value: torch.Tensor
     become the slots' scores. Slots past a row's count are left as they are.
 
     Args:
-        key, value: ``[T, Hkv, D]`` (any strides) in the cache's dtype.
+        key, value: ``[T, Hkv, D]`` (any strides) in the cache's dtype, in memory apart from the cache's.
         mass: fp32 ``[Hkv, T]`` (:func:`~economize_amd.prompt.attention_mass`).
         cu_seqlens: One sequence per cache row: ``cu_seqlens`` or ``(begin, end)``.
         max_seqlen: The longest sequence.

@@ -41,9 +41,11 @@ def row_bounds(rows: Rows, device: torch.device) -> tuple[object, int, int, int]
             raise ConfigError(f"cu_seqlens on {rows.device}, the queries on {device}")
         at = rows.data_ptr()
         return rows, at, at + 4, rows.numel() - 1
+    if not isinstance(rows, (tuple, list)) or len(rows) != 2:
+        raise ConfigError("sequences are given by cu_seqlens or by (begin, end)")
     begin, end = rows
     for t in (begin, end):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 1 or t.stride(0) != 1 or t.device != device:
+        if not torch.is_tensor(t) or t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 1 or t.stride(0) != 1 or t.device != device:
             raise ConfigError(f"begin and end must be contiguous int32 [sequences] on {device}")
     if begin.numel() != end.numel():
         raise ConfigError(f"{begin.numel()} sequences begin, {end.numel()} end")
@@ -73,6 +75,11 @@ def check_out(out: torch.Tensor, like: torch.Tensor, what: str) -> tuple[int, in
     same, at, a, b = operand(out)
     if same is not out:
         raise ConfigError(f"out must be {what}, channels contiguous and rows on 16 bytes")
+    reach = out.shape[2]  # elements up to the end of one entry of the axis before
+    for stride, n in sorted(((a, out.shape[0]), (b, out.shape[1]))):
+        if n > 1 and stride < reach:
+            raise ConfigError(f"out must be {what} with every element apart, not strides {tuple(out.stride())}")
+        reach += (n - 1) * stride
     return at, a, b
 
 
@@ -126,7 +133,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         max_seqlen_k: The longest sequence's keys.
         softcap: Optional tanh soft cap of the scaled scores.
         sinks: Optional ``[Hq]`` attention-sink logits.
-        out: Optional ``[T, Hq, D]`` output buffer; rows of no sequence are left as they are.
+        out: Optional ``[T, Hq, D]`` output buffer apart from the keys and values; rows of no sequence are left as they are.
         return_lse: Also return the logarithm of every softmax denominator, fp32 ``[Hq, T]``.
 
     Returns:

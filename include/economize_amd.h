@@ -505,7 +505,7 @@ int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h
  *
  * Fills it from packed prompts, row b from key rows [begin[b], end[b]): of its n tokens every KV head keeps all if they
  * fit, else the first, the newest and those of greatest mass [Hkv, sm_h] among the rest (equal: the lower index; a NaN is
- * the least), in token order. Slots past the count are left as they are. max_tokens bounds nothing but the launch. */
+ * the least), in token order. Slots past the count are left as they are. max_tokens sizes the launch. */
 int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
                      const float* mass, int64_t sm_h, const int32_t* begin, const int32_t* end, int64_t rows,
                      int32_t max_tokens, void* keys, void* values, float* score, int32_t* position, int32_t* count,

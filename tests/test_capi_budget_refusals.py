@@ -54,6 +54,9 @@ CASES = [
     ("eco_prompt_attention", dict(max_keys=30000, workspace_bytes=0), "workspace is too small"),
     ("eco_prompt_attention", dict(sequences=40000), "too many sequences"),
     ("eco_prompt_attention", dict(q_rows=1 << 30, sl_h=1 << 30), "too many queries"),
+    ("eco_prompt_attention", dict(so_t=0), "outputs overlap each other"),
+    ("eco_prompt_attention", dict(so_t=64, so_h=1920 - 8), "outputs overlap each other"),
+    ("eco_prompt_attention", dict(k_rows=0x7fffffff), "rows must be"),
     ("eco_attention_mass", dict(lse=None), "null pointer"),
     ("eco_attention_mass", dict(max_queries=30000, max_keys=30000), "workspace is too small"),
     ("eco_attention_mass", dict(window=-1), "must not be negative"),
@@ -65,6 +68,9 @@ CASES = [
     ("eco_evict_prompt", dict(recent=61), "recent \\+ first <= slots"),
     ("eco_evict_prompt", dict(slots=0), "sizes must be positive"),
     ("eco_evict_prompt", dict(slots=1 << 29), "too many slots"),
+    ("eco_evict_prompt", dict(batch=1, kv_heads=1, slots=(1 << 25) + 1), "too many slots"),
+    ("eco_evict_prompt", dict(batch=40000), "too many rows"),
+    ("eco_evict_prompt", dict(keys=FAKE - 64), "apart from the cache"),
     ("eco_evict_prompt", dict(sm_h=3), "mass rows are shorter"),
     ("eco_evict_prompt", dict(rows=-1), "rows must be"),
     ("eco_heavy_hitter_decode", dict(workspace=None), "null pointer"),
@@ -74,6 +80,8 @@ CASES = [
     ("eco_heavy_hitter_decode", dict(keys=FAKE + 2), "cache must be 16-byte aligned"),
     ("eco_heavy_hitter_decode", dict(head_dim=512), "head dim must be 64, 128 or 256"),
     ("eco_heavy_hitter_decode", dict(sk_b=4), "keys need strides"),
+    ("eco_heavy_hitter_decode", dict(so_h=32), "outputs overlap each other"),
+    ("eco_heavy_hitter_decode", dict(batch=70000, kv_heads=1, q_heads=1, slots=12), "too many rows"),
 ]
 
 
@@ -122,12 +130,16 @@ def test_workspaces() -> None:
     assert lib.eco_heavy_hitter_workspace_size(2, 8, 2, 64, 64) > 0
     assert lib.eco_heavy_hitter_workspace_size(2, 7, 2, 64, 64) == 0
     assert lib.eco_prompt_attention_workspace_size(2, 20, 10, 10, 7, 2, 64) == 0
+    # few rows in a large buffer: the parts' places for all of its rows stay within half a GiB
+    assert 0 < lib.eco_prompt_attention_workspace_size(1, 100, 100, 32768, 32, 8, 128) <= 1 << 29
+    assert 0 <= lib.eco_prompt_attention_workspace_size(1, 32768, 100, 32768, 32, 8, 128) <= 1 << 29
+    assert lib.eco_prompt_attention_workspace_size(1, 0, 0, 32768, 32, 8, 128) == 0
 
 
 def test_caches_and_rows_are_checked() -> None:
     from economize_amd.errors import ConfigError
     from economize_amd.eviction import HeavyHitterCache
-    from economize_amd.prompt import prompt_attention, row_bounds
+    from economize_amd.prompt import check_out, prompt_attention, row_bounds
 
     with pytest.raises(ConfigError, match="recent"):
         HeavyHitterCache.empty(1, 1, 64, 8, torch.bfloat16, "cpu", recent=9)
@@ -139,7 +151,14 @@ def test_caches_and_rows_are_checked() -> None:
     cpu = torch.device("cpu")
     cu = torch.tensor([0, 3, 3, 8], dtype=torch.int32)
     assert row_bounds(cu, cpu)[1:] == (cu.data_ptr(), cu.data_ptr() + 4, 3)
-    for rows in (cu.long(), cu[:1], cu[::2], cu[None], (cu, cu[:2]), (cu, cu.float())):
+    x = torch.zeros(6, 4, 64, dtype=torch.float16)
+    for out in (x, x[:, :2], x.transpose(0, 1).contiguous().transpose(0, 1), x[:1], x[:, :1]):
+        assert check_out(out, out, "") == (out.data_ptr(), *(s if n > 1 else t for n, s, t in zip(
+            out.shape, out.stride(), check_out(out, out, "")[1:])))
+    for out in (x[:1].expand(6, 4, 64), x[:, :1].expand(6, 4, 64), x.as_strided((3, 4, 64), (128, 64, 1)), x[..., ::2]):
+        with pytest.raises(ConfigError, match="out must be"):
+            check_out(out, out, "")
+    for rows in (cu.long(), cu[:1], cu[::2], cu[None], (cu, cu[:2]), (cu, cu.float()), (cu,), [0, 8], 8):
         with pytest.raises(ConfigError):
             row_bounds(rows, cpu)
     with pytest.raises(RuntimeError, match="AMD GPU"):

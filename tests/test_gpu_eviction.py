@@ -93,6 +93,24 @@ def test_evict_views_and_slots_past_the_count() -> None:
         assert torch.equal(cache.values[1, h], v[torch.from_numpy(90 + kept).cuda(), h])
 
 
+def test_evict_bound_and_own_memory() -> None:
+    """``max_seqlen`` sizes the launch: longer rows are copied all the same. A cache is no source of its own prompt."""
+    from economize_amd.errors import ConfigError
+    from economize_amd.eviction import HeavyHitterCache, evict_prompt
+
+    lens = [900, 1, 300]
+    _, k, v, cu, _ = prompt_inputs(27, lens, lens, (2, 2), 64, BF16)
+    mass = torch.rand(2, sum(lens), generator=torch.Generator().manual_seed(28)).cuda()
+    for bound in (0, 1, 40, 900, 10 ** 6, None):
+        cache = HeavyHitterCache.empty(3, 2, 64, 512, BF16, "cuda", 8, 4)
+        evict_prompt(cache, k, v, mass, cu, bound)
+        check_evicted(cache, k, v, mass, cu)
+    own = cache.keys[0].transpose(0, 1)
+    for args in ((own, v[:512], mass[:, :512]), (k[:512], own, mass[:, :512]), (k[:512], v[:512], cache.score[0])):
+        with pytest.raises(ConfigError, match="apart from the cache"):
+            evict_prompt(cache, *args, cu)
+
+
 def make_cache(seed, batch, heads, dim, dtype, budget, recent, first, seen):
     """A cache whose rows have seen ``seen`` tokens, the kept ones in mixed slots."""
     from economize_amd.eviction import HeavyHitterCache

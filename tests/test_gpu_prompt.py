@@ -112,6 +112,29 @@ def test_few_queries_behind_many_keys(lens_q, lens_k, dtype, dim) -> None:
     assert (out[-5:] == 2).all()
 
 
+@pytest.mark.parametrize("lens_q,lens_k,heads", [([70, 3], [6200, 900], (64, 2)), ([40], [6400], (64, 64))])
+def test_many_heads_over_many_keys(lens_q, lens_k, heads) -> None:
+    """Enough tiles of keys for 64 of them to a wave of the mass, cut by heads and whole."""
+    q, k, v, cu_q, cu_k = prompt_inputs(25, lens_q, lens_k, heads, 128, BF16)
+    check(q, k, v, cu_q, cu_k, lens_q, lens_k)
+
+
+def test_few_rows_of_a_large_buffer() -> None:
+    """One chunk in a buffer of many rows: what the rest holds does not matter, and it gives 0."""
+    q, k, v, _, _ = prompt_inputs(26, [6000], [6000], (4, 2), 64, BF16)
+    q[40:] = math.nan
+    k[5000:] = math.nan
+    v[5000:] = math.nan
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows, rows_k = (zero, zero + 40), (zero, zero + 5000)
+    from economize_amd.prompt import prompt_attention
+    out, lse = prompt_attention(q, k, v, rows, 40, cu_seqlens_k=rows_k, max_seqlen_k=5000, return_lse=True)
+    assert not out[40:].any() and torch.isneginf(lse[:, 40:]).all()
+    cu = np.array([0, 40]), np.array([0, 5000])
+    exact, _, size = ob.prompt_attention(f64(q[:40]), f64(k[:5000]), f64(v[:5000]), *cu, 64 ** -0.5)
+    assert_output(out[:40], exact, size, score_error(q[:40], k[:5000], 64 ** -0.5, 5000))
+
+
 def test_unseen_nan_in_a_cut_row() -> None:
     """The keys are cut, and the last tiles hold infinities that only the last queries see."""
     q, k, v, cu_q, cu_k = prompt_inputs(18, [100], [3000], (4, 2), 128, BF16)
