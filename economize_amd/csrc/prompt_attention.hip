@@ -405,7 +405,8 @@ int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int
 template <int D, int FMT>
 int launch(PromptParams p, int max_queries, int max_keys, hipStream_t stream) {
     const int64_t tiles = (static_cast<int64_t>(max_queries) * p.groups + ROWS - 1) / ROWS;
-    const int64_t bytes = static_cast<int64_t>(max_keys) * D * 4;
+    // (twice the average where the longest is not known: 24 prompts, 24572 keys: 369 us, 381 as if each had them all)
+    const int64_t twice = 2 * p.rows.k_rows / p.rows.sequences, bytes = (twice < max_keys ? twice : max_keys) * D * 4;
     p.order = work_order(p.rows.sequences, p.kv_heads, tiles, p.parts, bytes);
     p.per_group = Divisor(p.groups);
     p.per_kv = Divisor(p.kv_heads);

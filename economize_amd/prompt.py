@@ -34,13 +34,14 @@ STRIDE_LIMIT = 1 << 24
 def row_bounds(rows: Rows, device: torch.device) -> tuple[object, int, int, int]:
     """What keeps the bounds alive, the addresses of every sequence's first and past-the-end row, and how many sequences
     there are."""
-    if torch.is_tensor(rows):
-        if rows.dtype is not torch.int32 or rows.dim() != 1 or rows.numel() < 2 or rows.stride(0) != 1:
+    if isinstance(rows, torch.Tensor):
+        shape = rows.shape
+        if rows.dtype is not torch.int32 or len(shape) != 1 or shape[0] < 2 or not rows.is_contiguous():
             raise ConfigError("cu_seqlens must be contiguous int32 [sequences + 1] with at least one sequence")
         if rows.device != device:
             raise ConfigError(f"cu_seqlens on {rows.device}, the queries on {device}")
         at = rows.data_ptr()
-        return rows, at, at + 4, rows.numel() - 1
+        return rows, at, at + 4, shape[0] - 1
     if not isinstance(rows, (tuple, list)) or len(rows) != 2:
         raise ConfigError("sequences are given by cu_seqlens or by (begin, end)")
     begin, end = rows
@@ -83,14 +84,18 @@ def check_out(out: torch.Tensor, like: torch.Tensor, what: str) -> tuple[int, in
     return at, a, b
 
 
-def _check(what: str, query: torch.Tensor, key: torch.Tensor) -> None:
-    if query.dim() != 3 or key.dim() != 3 or query.shape[2] != key.shape[2]:
-        raise ConfigError(f"{what} takes queries [T, Hq, D] and keys [Tk, Hkv, D], got {tuple(query.shape)} and "
-                          f"{tuple(key.shape)}")
-    if query.dtype not in DTYPES or key.dtype != query.dtype:
-        raise ConfigError(f"{what} takes bf16 or fp16 queries and keys of one dtype, got {query.dtype} and {key.dtype}")
-    if key.shape[1] == 0 or query.shape[1] % key.shape[1] or query.shape[1] == 0:
-        raise ConfigError(f"{query.shape[1]} query heads are not a multiple of {key.shape[1]} KV heads")
+def _check(what: str, query: torch.Tensor, key: torch.Tensor) -> tuple[int, int, int, int, int, int]:
+    """Queries, query heads, head dim, keys, KV heads and the C ABI's format."""
+    shape, shape_k, dtype = query.shape, key.shape, query.dtype
+    if len(shape) != 3 or len(shape_k) != 3 or shape[2] != shape_k[2]:
+        raise ConfigError(f"{what} takes queries [T, Hq, D] and keys [Tk, Hkv, D], got {tuple(shape)} and {tuple(shape_k)}")
+    if dtype not in DTYPES or key.dtype is not dtype:
+        raise ConfigError(f"{what} takes bf16 or fp16 queries and keys of one dtype, got {dtype} and {key.dtype}")
+    tokens, q_heads, head_dim = shape
+    keys, kv_heads, _ = shape_k
+    if kv_heads == 0 or q_heads % kv_heads or q_heads == 0:
+        raise ConfigError(f"{q_heads} query heads are not a multiple of {kv_heads} KV heads")
+    return tokens, q_heads, head_dim, keys, kv_heads, _lib.fmt(dtype)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -141,11 +146,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         ``out`` a row of no sequence, gives 0 and ``-inf``. Nothing here is differentiated.
     """
     device = _lib.require_gpu(query, key, value)
-    _check("prompt_attention", query, key)
-    if value.shape != key.shape or value.dtype != key.dtype:
+    tokens, q_heads, head_dim, keys, kv_heads, form = _check("prompt_attention", query, key)
+    if value.shape != key.shape or value.dtype is not key.dtype:
         raise ConfigError(f"values {tuple(value.shape)} {value.dtype} do not match the keys {tuple(key.shape)} {key.dtype}")
-    tokens, q_heads, head_dim = query.shape
-    keys, kv_heads, _ = key.shape
     (keep, q_begin, q_end, sequences), (keep_k, k_begin, k_end, _) = _sequences(cu_seqlens, cu_seqlens_k, tokens, keys,
                                                                                 device)
     if sinks is not None:
@@ -172,7 +175,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         need = _prompt_workspace(sequences, tokens, max_q, max_k, q_heads, kv_heads, head_dim)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         _lib.call_on(
-            device, "eco_prompt_attention", q_at, _lib.fmt(query.dtype), sq_t, sq_h, k_at, v_at, sk_t, sk_h, sv_t, sv_h,
+            device, "eco_prompt_attention", q_at, form, sq_t, sq_h, k_at, v_at, sk_t, sk_h, sv_t, sv_h,
             q_begin, q_end, k_begin, k_end, sequences, tokens, keys, max_q, max_k, _lib.ptr(sinks), at, so_t, so_h,
             _lib.ptr(lse), tokens, fill, q_heads, kv_heads, head_dim, head_dim ** -0.5 if scale is None else scale,
             softcap or 0.0, _lib.ptr(ws), need)
@@ -194,14 +197,12 @@ def attention_mass(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu
         out: Optional fp32 ``[Hkv, Tk]`` output buffer; keys of no sequence are left as they are (without it they give 0).
     """
     device = _lib.require_gpu(query, key, lse)
-    _check("attention_mass", query, key)
-    tokens, q_heads, head_dim = query.shape
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (q_heads, tokens) or (tokens > 1 and lse.stride(1) != 1) or \
+    tokens, q_heads, head_dim, keys, kv_heads, form = _check("attention_mass", query, key)
+    if lse.dtype is not torch.float32 or lse.shape != (q_heads, tokens) or (tokens > 1 and lse.stride(1) != 1) or \
             (q_heads > 1 and lse.stride(0) < tokens):
         raise ConfigError(f"lse must be fp32 [{q_heads}, {tokens}] with contiguous rows apart")
     if window is not None and (isinstance(window, bool) or int(window) != window or window < 1):
         raise ConfigError(f"window must be a positive integer or None, got {window!r}")
-    keys, kv_heads, _ = key.shape
     (keep, q_begin, q_end, sequences), (keep_k, k_begin, k_end, _) = _sequences(cu_seqlens, cu_seqlens_k, tokens, keys,
                                                                                 device)
     fill = out is None
@@ -219,7 +220,7 @@ def attention_mass(query: torch.Tensor, key: torch.Tensor, lse: torch.Tensor, cu
         need = _mass_workspace(max_q, keys, window, q_heads, kv_heads)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         _lib.call_on(
-            device, "eco_attention_mass", q_at, _lib.fmt(query.dtype), sq_t, sq_h, k_at, sk_t, sk_h, lse.data_ptr(),
+            device, "eco_attention_mass", q_at, form, sq_t, sq_h, k_at, sk_t, sk_h, lse.data_ptr(),
             lse.stride(0) if q_heads > 1 else tokens, q_begin, q_end, k_begin, k_end, sequences, tokens, keys, max_q, max_k,
             window, out.data_ptr(), out.stride(0) if kv_heads > 1 else keys, fill, q_heads, kv_heads, head_dim,
             head_dim ** -0.5 if scale is None else scale, softcap or 0.0, _lib.ptr(ws), need)
