@@ -41,7 +41,7 @@ __global__ __launch_bounds__(THREADS, KT == 2 || D == 256 ? 2 : D == 128 ? 4 : 5
     if (!work_of(p.order, blockIdx.x, pair, slot)) return;
     const int first = p.per_part(slot), part = slot - first * p.parts, stride = p.order.tiles / p.parts;
     const int s = p.per_kv(pair), kvh = pair - s * p.kv_heads;
-    const Sequence seq = sequence_of(p.rows, s);
+    const Sequence seq = ranked_sequence(p.rows, s);
     const int tiles = (seq.nk + KEYS - 1) / KEYS;
     const int offset = seq.nk - seq.nq;
     const int window_begin = p.window > 0 && p.window < seq.nq ? seq.nq - p.window : 0;

@@ -29,6 +29,9 @@ struct Divisor {
 // Workgroups that look after the rows of no sequence, where a call asks for it.
 constexpr int FILLERS = 128;
 
+// Up to so many sequences are taken by their work, the most first.
+constexpr int SORTED = 8;
+
 // Which (sequence, KV head) pair and which of its tiles a workgroup takes. The tiles of a pair read the same rows, so they
 // run close together: the pairs in `group` at a time, their longest tiles first. Workgroups go to the eight XCDs in turn,
 // each with an L2 of its own: with `pin` a pair stays on one.

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : D == 128 ? 2 : 3) void prom
     // (parts outermost: workgroups without work come last, where they leave no shader engine without any)
     const int stride = p.per_part.by, part = p.per_part(slot), first = slot - part * stride;
     const int s = p.per_kv(pair), kvh = pair - s * p.kv_heads;
-    const Sequence seq = sequence_of(p.rows, s);
+    const Sequence seq = ranked_sequence(p.rows, s);
     const int total = seq.nq * p.groups;  // (below 2^31: the host checks)
     const int tiles = (total + ROWS - 1) / ROWS;
     const int offset = seq.nk - seq.nq;  // query i sees keys <= i + offset

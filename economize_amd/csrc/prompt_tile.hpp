@@ -61,6 +61,30 @@ __device__ __forceinline__ Sequence sequence_of(const PackedRows& r, int s) {
     return q;
 }
 
+// The sequence of this rank by work, the most first, where there are few: the last workgroups are then short ones (6 prompt
+// chunks 143 -> 131 us, the masses of 4 prompts 500 -> 460 us). Many even out in any order and lose by it
+// (24 packed prompts 376 -> 389 us, the last queries of 16 29.4 -> 30.5). Every lane holds one sequence's bounds and counts
+// those before it.
+__device__ __forceinline__ Sequence ranked_sequence(const PackedRows& r, int rank) {
+    if (r.sequences == 1 || r.sequences > SORTED) return sequence_of(r, rank);
+    const int lane = threadIdx.x & 63;
+    static_assert(SORTED <= 64, "a lane to each");
+    const Sequence mine = sequence_of(r, lane < r.sequences ? lane : r.sequences - 1);
+    const float work = static_cast<float>(mine.nq) * (2.0f * static_cast<float>(mine.nk) - static_cast<float>(mine.nq));
+    int before = 0;
+    for (int j = 0; j < r.sequences; ++j) {
+        const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(work), j));
+        before += other > work || (other == work && j < lane) ? 1 : 0;
+    }
+    const int from = __builtin_amdgcn_readfirstlane(__ffsll(__ballot(lane < r.sequences && before == rank)) - 1);
+    Sequence q;
+    q.q0 = __builtin_amdgcn_readlane(static_cast<int>(mine.q0), from);  // (rows are below 2^31)
+    q.k0 = __builtin_amdgcn_readlane(static_cast<int>(mine.k0), from);
+    q.nq = __builtin_amdgcn_readlane(mine.nq, from);
+    q.nk = __builtin_amdgcn_readlane(mine.nk, from);
+    return q;
+}
+
 // The pair and the tile (0 the longest) of workgroup id; false where there is none.
 __device__ __forceinline__ bool work_of(const WorkOrder& o, int id, int& pair, int& tile) {
     const int total = o.pin ? (o.pairs + 7) / 8 : o.pairs;
