@@ -1,13 +1,18 @@
-// The attention weight every key of packed prompts receives: mass[h, j] = sum over the queries i that see key j (all, or
-// the last `window` of its sequence) and the query heads of KV head h of exp(x_ij - lse_i), from the softmax statistics
-// lse_i the attention left: one product, no running maximum.
+// The attention weight every key of packed prompts receives: mass[h, j] = sum over the queries i that see key j (all,
+// or the last `window` of its sequence) and the query heads of KV head h of exp(x_ij - lse_i), from the softmax
+// statistics lse_i the attention left: one product, no running maximum.
 //
-// A wave holds 32 KT keys as columns in registers and streams the queries of the group's heads through LDS, 64 at a time:
-// S = Q K^T puts one key in each lane with 16 of 32 queries in its registers, so a weight is added where it is computed, in
-// fp32 and in a fixed order: no atomics, the same bits every time. The products of 32 queries run while the weights of the
-// 32 before are computed. All tiles of a (sequence, KV head) walk the queries from the last down, so they read the same ones
-// at the same time. Long walks are cut by
-// heads, each a workgroup of its own, summed by mass_sum_kernel.
+// A wave holds 32 KT keys as columns in registers and streams the queries of the group's heads through LDS, 64 at a
+// time: S = Q K^T puts one key in each lane with 16 of 32 queries in its registers, so a weight is added where it is
+// computed, in fp32 and in a fixed order: no atomics, the same bits every time. The products of 32 queries run while
+// the weights of the 32 before are computed. All tiles of a (sequence, KV head) walk the queries from the last down, so
+// they read the same ones at the same time. Long walks are cut by heads, each a workgroup of its own, summed by
+// mass_sum_kernel.
+//
+// Bound by the matrix instructions and the exponentials together: 32768 tokens, 32 heads of 128 on 8, take 3.9 ms, 1.13
+// PFLOP/s (1.31 in a large library product); 4 prompts of 1000 to 8192 tokens 460 us, 1.01. The last 64 queries of 16
+// prompts of 501 to 8000 tokens (16 heads of 64 on 4) take 29 us, four times their keys' HBM time: four steps to a
+// walk, whose fetches and barriers a workgroup waits for.
 
 #include "prompt_tile.hpp"
 
@@ -191,9 +196,9 @@ __global__ __launch_bounds__(256) void mass_sum_kernel(MassParams p) {
     }
 }
 
-// Long walks are cut by heads: their lengths differ up to the whole, and shorter ones even out (one prompt of 500 tokens,
-// 32 heads of 128 on 8: 40 us whole, 16 us cut). A window's walks are as long as each other and only gain from being many
-// (window 256 over 16 x 4200 keys: 151 us whole, 167 cut; window 512 over 30000: 151 and 135).
+// Long walks are cut by heads: their lengths differ up to the whole, and shorter ones even out (one prompt of 500
+// tokens, 32 heads of 128 on 8: 40 us whole, 16 us cut). A window's walks are as long as each other and only gain from
+// being many (window 256 over 16 x 4200 keys: 151 us whole, 167 cut; window 512 over 30000: 151 and 135).
 int parts_of(int max_queries, bool windowed, int groups) {
     const int64_t steps = (static_cast<int64_t>(max_queries) + 63) / 64 * groups;
     return steps >= (windowed ? 32 : 12) ? groups : 1;
@@ -223,9 +228,9 @@ int launch(MassParams p, int max_queries, int max_keys, hipStream_t stream) {
 }
 
 // Keys to a wave: 32, or 64 of 128 channels, for which every query fragment read from LDS feeds two products, where six
-// workgroups to a CU are left. With 32 and 64: 1 x 4000 tokens, 32 heads on 8: 91 and 113 us; 8 x 1000: 55 and 65; 8 x 4000:
-// 586 and 566; 1 x 16000: 1045 and 982. Heads of 64 channels are bound by the exponentials, and more waves hide more of the
-// rest (1 x 16000 tokens, 16 heads on 4: 407 and 474 us); 256 channels leave no registers for more.
+// workgroups to a CU are left. With 32 and 64: 1 x 4000 tokens, 32 heads on 8: 91 and 113 us; 8 x 1000: 55 and 65; 8 x
+// 4000: 586 and 566; 1 x 16000: 1045 and 982. Heads of 64 channels are bound by the exponentials, and more waves hide
+// more of the rest (1 x 16000 tokens, 16 heads on 4: 407 and 474 us); 256 channels leave no registers for more.
 template <int FMT>
 int launch_dim(const MassParams& p, int max_queries, int max_keys, hipStream_t stream) {
     if (p.head_dim == 64) return launch<64, FMT, 1>(p, max_queries, max_keys, stream);

@@ -1,6 +1,6 @@
-// Cutting packed prompts to a cache's budget: of the n tokens of a row, every KV head keeps all if they fit C slots, else
-// the first `first`, the newest `recent` and the C - first - recent of greatest mass among the rest (equal masses: the
-// lower index), in token order.
+// Cutting packed prompts to a cache's budget: of the n tokens of a row, every KV head keeps all if they fit C slots,
+// else the first `first`, the newest `recent` and the C - first - recent of greatest mass among the rest (equal masses:
+// the lower index), in token order.
 
 #include "eviction.hpp"
 
@@ -15,10 +15,10 @@ constexpr int COPIES = 4;   // of the histogram: lanes of equal digits would que
 constexpr int BINS = 2048, COPY = BINS + 4;  // (a bin's copies lie in different banks)
 
 // One workgroup per (row, KV head): the mass of the last token to keep by a radix selection over its 32 bits (digits of
-// 11, 11 and 10 bits, histograms in LDS), then the kept tokens' positions and masses in order. Up to HELD THREADS tokens
-// are read once; longer rows once per digit and once more for the kept ones.
-// Bound by its dependent rounds, not by the 4 bytes a token: 16 rows of 8 heads of 6000 to 8192 tokens take 15 us (one
-// histogram and one load at a time: 18 us), a row of 1021 tokens 8.
+// 11, 11 and 10 bits, histograms in LDS), then the kept tokens' positions and masses in order. Up to HELD THREADS
+// tokens are read once; longer rows once per digit and once more for the kept ones. Bound by its dependent rounds, not
+// by the 4 bytes a token: 16 rows of 8 heads of 6000 to 8192 tokens take 15 us (one histogram and one load at a time:
+// 18 us), a row of 1021 tokens 8.
 __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictParams p) {
     __shared__ __align__(16) uint32_t hist[COPY * COPIES];
     __shared__ uint32_t counts[HELD][WAVES];  // tokens above the last one to keep, and equal to it << 16
@@ -171,7 +171,9 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictParams p) {
     }
 }
 
-// The kept tokens' keys and values: one 16-byte chunk per thread, where the launch holds the longest row.
+// The kept tokens' keys and values: one 16-byte chunk per thread, where the launch holds the longest row. Bound by HBM
+// (16 rows of 8 heads, 1024 kept of 128 channels: 27 us for 135 MB, 5.0 TB/s); the 15 us of the selection come before
+// it.
 __global__ __launch_bounds__(256) void evict_copy_kernel(EvictParams p) {
     const BudgetCache& c = p.cache;
     const int chunks = c.head_dim / 8;

@@ -1,14 +1,18 @@
-// One decode step over a cache held at a budget. The row's new token takes the next free slot, or, when all C are filled,
-// the slot of lowest score among those whose token is neither one of the first nor one of the newest (equal scores: the
-// lower slot). The token's query heads attend over every filled slot, and each slot's score grows by the weight it
-// received, summed over the heads of its KV head.
+// One decode step over a cache held at a budget. The row's new token takes the next free slot, or, when all C are
+// filled, the slot of lowest score among those whose token is neither one of the first nor one of the newest (equal
+// scores: the lower slot). The token's query heads attend over every filled slot, and each slot's score grows by the
+// weight it received, summed over the heads of its KV head.
 //
-// heavy_attend_kernel: a row's slots are cut into parts, one workgroup each; a wave takes 32 slots at a time, its 16 query
-// heads as columns (S^T = K Q^T, v_mfma_f32_16x16x32: one head per lane), so P^T is the second product's operand with
-// values read transposed from LDS. The scaled scores go to the workspace with the part's maximum, sum and outputs.
-// heavy_merge_kernel: the parts' join, and the weights from the scores kept, added to the slots' scores. Every sum has a
-// fixed order: no atomics. (The join by the last part of a row to finish, in the same launch, took as long for 2048 slots of
-// 4 heads, 57.6 us against 55.0, and twice as long for one row of 8192, 83 against 44.)
+// heavy_attend_kernel: a row's slots are cut into parts, one workgroup each; a wave takes 32 slots at a time, its 16
+// query heads as columns (S^T = K Q^T, v_mfma_f32_16x16x32: one head per lane), so P^T is the second product's operand
+// with values read transposed from LDS. The scaled scores go to the workspace with the part's maximum, sum and outputs.
+// heavy_merge_kernel: the parts' join, and the weights from the scores kept, added to the slots' scores. Every sum has
+// a fixed order: no atomics. (The join by the last part of a row to finish, in the same launch, took as long for 2048
+// slots of 4 heads, 57.6 us against 55.0, and twice as long for one row of 8192, 83 against 44.)
+//
+// Bound by HBM: 32 rows of 8 heads and up to 2048 slots of 128 channels take 42 us in the first kernel (5.4 TB/s) and 5
+// in the second, 58 us a call; 16 rows of 16 heads and 4096 slots of 256 channels 169 us (6.3 TB/s) and 5. One row of a
+// small model (8 heads of 64 on 2, 512 slots) takes 7 and 3 us on the GPU, 15 us a call with the host's part.
 
 #include "eviction.hpp"
 
@@ -312,8 +316,8 @@ __device__ __forceinline__ float2 head_stats(const HeavyParams& p, int bh, int g
     return make_float2(most, sum);
 }
 
-// The parts' join: the first p.groups workgroups of a row and KV head give one head's output each, the others the scores of
-// 4 THREADS slots each.
+// The parts' join: the first p.groups workgroups of a row and KV head give one head's output each, the others the
+// scores of 4 THREADS slots each.
 template <int D, int FMT>
 __global__ __launch_bounds__(THREADS) void heavy_merge_kernel(HeavyParams p) {
     const BudgetCache& c = p.cache;
@@ -394,9 +398,10 @@ struct Plan {
 Plan make_plan(int batch, int q_heads, int kv_heads, int slots, int head_dim) {
     Plan r;
     const int64_t groups = q_heads / kv_heads, rows = static_cast<int64_t>(batch) * kv_heads;
-    // as many workgroups as are resident at once on 256 CUs: one per CU at head dim 256 (its tiles fill the LDS), two below
-    // (16 rows of 16 heads and 4096 slots of 256 channels: 177 us at one, 182 at two, 198 at four; 32 rows of 8 heads and 2048
-    // of 128: 59 at one, 58 at two, 61 at four, 66 at six), but at least 128 slots (a step of the four waves) to each
+    // as many workgroups as are resident at once on 256 CUs: one per CU at head dim 256 (its tiles fill the LDS), two
+    // below (16 rows of 16 heads and 4096 slots of 256 channels: 177 us at one, 182 at two, 198 at four; 32 rows of 8
+    // heads and 2048 of 128: 59 at one, 58 at two, 61 at four, 66 at six), but at least 128 slots (a step of the four
+    // waves) to each
     const int64_t per_cu = head_dim == 256 ? 1 : 2;
     int64_t splits = (per_cu * 256 + rows - 1) / rows;
     const int64_t most = (slots + 127) / 128;
@@ -452,9 +457,9 @@ int heavy_hitter_decode(HeavyParams p, int format, void* workspace, size_t works
     p.splits = r.splits;
     p.span = r.span;
     p.pitch = r.pitch;
-    // Every workgroup reading all scores and positions of its row costs less than a launch until there are many of both (one
-    // row of 8 heads: 8192 slots 17 us either way, 32768 slots 36 us against 40, 131072 slots 129 against 158; 32 rows of 2048
-    // slots 60 against 57).
+    // Every workgroup reading all scores and positions of its row costs less than a launch until there are many of both
+    // (one row of 8 heads: 8192 slots 17 us either way, 32768 slots 36 us against 40, 131072 slots 129 against 158; 32
+    // rows of 2048 slots 60 against 57).
     p.chosen = c.slots >= 16384;
     return format == BF16 ? launch_dim<BF16>(p, stream) : launch_dim<FP16>(p, stream);
 }

@@ -32,9 +32,9 @@ constexpr int FILLERS = 128;
 // Up to so many sequences are taken by their work, the most first.
 constexpr int SORTED = 8;
 
-// Which (sequence, KV head) pair and which of its tiles a workgroup takes. The tiles of a pair read the same rows, so they
-// run close together: the pairs in `group` at a time, their longest tiles first. Workgroups go to the eight XCDs in turn,
-// each with an L2 of its own: with `pin` a pair stays on one.
+// Which (sequence, KV head) pair and which of its tiles a workgroup takes. The tiles of a pair read the same rows, so
+// they run close together: the pairs in `group` at a time, their longest tiles first. Workgroups go to the eight XCDs
+// in turn, each with an L2 of its own: with `pin` a pair stays on one.
 struct WorkOrder {
     int pairs, tiles, group, pin;
     Divisor whole, full_width, last_width;  // workgroups of a group of pairs; pairs in a group, and in the last one
@@ -42,9 +42,10 @@ struct WorkOrder {
     int64_t blocks() const { return static_cast<int64_t>(tiles) * (pin ? 8 * per_xcd() : pairs); }
 };
 
-// `tiles` of `parts` workgroups each per pair, whose rows read by all of them take `bytes`: as many pairs at a time as three quarters of an L2 hold.
-// Pinned where that leaves the XCDs about the same work: with KV heads in eights each gets every sequence, otherwise many
-// sequences even out (6 sequences of different lengths with 4 KV heads, pinned: half of the CUs' time idle).
+// `tiles` of `parts` workgroups each per pair, whose rows read by all of them take `bytes`: as many pairs at a time as
+// three quarters of an L2 hold. Pinned where that leaves the XCDs about the same work: with KV heads in eights each
+// gets every sequence, otherwise many sequences even out (6 sequences of different lengths with 4 KV heads, pinned:
+// half of the CUs' time idle).
 inline WorkOrder work_order(int sequences, int kv_heads, int64_t tiles, int parts, int64_t bytes) {
     const int64_t pairs = static_cast<int64_t>(sequences) * kv_heads;
     const int64_t most_tiles = (1 << 23) / (pairs * parts);

@@ -1,14 +1,22 @@
 // Attention over packed prompts: every sequence's queries attend causally over its own keys.
 //
-// With x_ij = scale q_i . k_j (soft-capped or not), query i gives o_i = sum_j exp(x_ij - lse_i) v_j over the keys it sees,
-// lse_i = log(sum_j exp(x_ij) + exp(sink)). One pass over the keys with a running maximum and sum (both fp32).
+// With x_ij = scale q_i . k_j (soft-capped or not), query i gives o_i = sum_j exp(x_ij - lse_i) v_j over the keys it
+// sees, lse_i = log(sum_j exp(x_ij) + exp(sink)). One pass over the keys with a running maximum and sum (both fp32).
 //
 // A workgroup holds 128 rows of one (sequence, KV head): row r is query r / G of head r % G of the group, so the G
-// heads of a group share every K/V tile and a tile's rows span few queries (little of the causal diagonal is wasted).
-// A wave holds 32 rows as columns: S^T = K Q^T puts one query in each lane (l % 32) with 16 of 32 keys in its
-// registers, so the softmax needs one exchange with lane l ^ 32 and P^T is already the second product's operand: its eight
-// keys per lane are {4 h .. 4 h + 3, 8 + 4 h ..} of 16 (h = l / 32), the order the transposed value reads deliver.
-// O^T keeps the query in the lane, so rescaling is one multiplier per lane.
+// heads of a group share every K/V tile and a tile's rows span few queries (little of the causal diagonal is wasted). A
+// wave holds 32 rows as columns: S^T = K Q^T puts one query in each lane (l % 32) with 16 of 32 keys in its registers,
+// so the softmax needs one exchange with lane l ^ 32 and P^T is already the second product's operand: its eight keys
+// per lane are {4 h .. 4 h + 3, 8 + 4 h ..} of 16 (h = l / 32), the order the transposed value reads deliver. O^T keeps
+// the query in the lane, so rescaling is one multiplier per lane. Keys and values come straight into LDS, two tiles of
+// 64 each, one step ahead; the scores of a tile are computed under the exponentials of the one before.
+//
+// Long sequences are bound by the matrix instructions and the power they draw: 32768 tokens, 32 heads of 128 on 8, take
+// 8.0 ms, 1.1 PFLOP/s (a large library product reaches 1.31; on zeros, which draw less, a build of 8.5 ms took 6.4).
+// Short ones are bound by a row tile's chain of bounds, keys, products and outputs (6 us beside 1.3 us a tile of keys):
+// 24 prompts of 1 to 2047 tokens take 366 us, 0.77 PFLOP/s. Heads of 64 are bound by the exponentials (8 x 4000 tokens:
+// 0.80 PFLOP/s), heads of 256 by registers, which leave one wave to a SIMD (0.59). 64 rows to a wave read LDS half as
+// often but left no registers to overlap products and exponentials (32768 tokens 10 ms where 32 rows took 8.5).
 
 #include "prompt_tile.hpp"
 
@@ -72,9 +80,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : D == 128 ? 2 : 3) void prom
     auto over_groups = [&](int r) { return p.per_group(r); };
     const float cc = CAP ? 1.0f : p.scale * kLog2e;
     const TileCopy<D, THREADS> kcopy(tid, p.sk_t, true), vcopy(tid, p.sv_t, false);
-    // Fragment places in a tile: keys row l % 32, 8 channels from 8 (l / 32); values transposed, rows 4 (l / 32) + l % 16 / 4,
-    // channels 16 (l / 16 % 2) + 4 (l % 4). The swizzles are exclusive-ors of the chunk, so the place of channel step i is the
-    // first one's with 32 i (values: 64 d) flipped, and further rows are a constant away.
+    // Fragment places in a tile: keys row l % 32, 8 channels from 8 (l / 32); values transposed, rows 4 (l / 32) + l %
+    // 16 / 4, channels 16 (l / 16 % 2) + 4 (l % 4). The swizzles are exclusive-ors of the chunk, so the place of
+    // channel step i is the first one's with 32 i (values: 64 d) flipped, and further rows are a constant away.
     const int vrow = 4 * half + ((lane & 15) >> 2);
     const uint32_t kplace = col * (D * 2) + T::key_chunk(col, half) * 16;
     const uint32_t vplace = vrow * (D * 2) + T::value_chunk(vrow, ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
@@ -190,8 +198,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : D == 128 ? 2 : 3) void prom
                     acc[d] = mfma32<FMT>(vf, make_uint4(pf[4 * b], pf[4 * b + 1], pf[4 * b + 2], pf[4 * b + 3]), acc[d]);
                 }
         };
-        // Tile j's values have arrived and are about to be used. A weight of 0 times an infinity or a NaN would be a NaN: in
-        // the tiles that some rows do not see whole such values become 0, and are added at the end to the rows that see them.
+        // Tile j's values have arrived and are about to be used. A weight of 0 times an infinity or a NaN would be a
+        // NaN: in the tiles that some rows do not see whole such values become 0, and are added at the end to the rows
+        // that see them.
         auto clean = [&](int j) {
             if (64 * j + 63 > full) {
                 if (clean_values<D, FMT, THREADS>(lds[2 + (j & 1)], tid)) unseen = 1;
@@ -315,7 +324,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : D == 128 ? 2 : 3) void prom
     }
 }
 
-// The parts of the rows whose keys were cut: four channels to a lane, JOINED rows of a row tile to a workgroup.
+// The parts of the rows whose keys were cut (6 prompt chunks of 100 to 612 tokens in two parts: 12 us of 131, at 2.5
+// TB/s): four channels to a lane, JOINED rows of a row tile to a workgroup.
 constexpr int JOINED = 32;
 
 template <int D, int FMT>
@@ -387,8 +397,10 @@ size_t part_bytes(int parts, int64_t q_rows, int q_heads, int floats) {
 // The parts' workspace has a place for every row, also where a few rows of a large buffer are sequences.
 constexpr int64_t MOST_PART_BYTES = 1 << 29;
 
-// Where there are too few row tiles for the GPU (six to a CU: prompt chunks of 6 sequences take 147 us at four, 142 at six,
-// 164 at sixteen), their keys are cut into up to so many parts.
+// Where there are fewer row tiles than workgroups resident at once (two to a CU; one at head dim 256, whose tiles fill
+// the LDS), their keys are cut into up to so many parts. With twice the workgroups and with these, 32 heads of 128 on 8:
+// a prompt of 4000 tokens 178 and 146 us, 512 tokens behind 8000 98 and 89, 128 behind 16000 82 and 63; 16 heads of 256:
+// a prompt of 2000 tokens 111 and 98, 512 behind 30000 410 and 376.
 int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads, int head_dim) {
     if (q_rows == 0) return 1;
     const int64_t groups = q_heads / kv_heads;
@@ -398,7 +410,8 @@ int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int
     int64_t most = static_cast<int64_t>(max_keys) / (64 * MIN_PART);
     const int64_t fit = MOST_PART_BYTES / static_cast<int64_t>(part_bytes(1, q_rows, q_heads, head_dim + 2));
     most = most < fit ? most : fit;
-    const int64_t parts = row_tiles > 0 ? (1536 + row_tiles - 1) / row_tiles : 1;
+    const int64_t resident = head_dim == 256 ? 256 : 512;
+    const int64_t parts = row_tiles > 0 ? (resident + row_tiles - 1) / row_tiles : 1;
     return static_cast<int>(parts < 1 || most < 1 ? 1 : parts < most ? parts : most);
 }
 

@@ -61,9 +61,9 @@ __device__ __forceinline__ Sequence sequence_of(const PackedRows& r, int s) {
     return q;
 }
 
-// The sequence of this rank by work, the most first, where there are few: the last workgroups are then short ones (6 prompt
-// chunks 143 -> 131 us, the masses of 4 prompts 500 -> 460 us). Many even out in any order and lose by it
-// (24 packed prompts 376 -> 389 us, the last queries of 16 29.4 -> 30.5). Every lane holds one sequence's bounds and counts
+// The sequence of this rank by work, the most first, where there are few: the last workgroups are then short ones (6
+// prompt chunks 143 -> 131 us, the masses of 4 prompts 500 -> 460 us). Many even out in any order and lose by it (24
+// packed prompts 376 -> 389 us, the last queries of 16 29.4 -> 30.5). Every lane holds one sequence's bounds and counts
 // those before it.
 __device__ __forceinline__ Sequence ranked_sequence(const PackedRows& r, int rank) {
     if (r.sequences == 1 || r.sequences > SORTED) return sequence_of(r, rank);
@@ -97,8 +97,9 @@ __device__ __forceinline__ bool work_of(const WorkOrder& o, int id, int& pair, i
     return pair < o.pairs;
 }
 
-// The rows of no sequence, by FILLERS workgroups, of which this is `me`: visit(from, to, worker, workers) for its share of
-// the gaps before, between and behind the sequences. (Gaps side by side: one after the other each costs a chain of two loads.)
+// The rows of no sequence, by FILLERS workgroups, of which this is `me`: visit(from, to, worker, workers) for its share
+// of the gaps before, between and behind the sequences. (Gaps side by side: one after the other each costs a chain of
+// two loads.)
 template <typename Visit>
 __device__ __forceinline__ void for_gaps(const int32_t* begin, const int32_t* end, int sequences, int64_t rows, int me, Visit visit) {
     const int gaps = sequences + 1, at_once = gaps < 32 ? gaps : 32;
@@ -114,8 +115,8 @@ __device__ __forceinline__ void for_gaps(const int32_t* begin, const int32_t* en
 }
 
 // A tile of 64 rows of D 16-bit channels in LDS, in chunks of 16 bytes. Keys are read as MFMA operands of 32 rows by 16
-// channels (ds_read_b128, lane l row l % 32), values transposed (ds_read_b64_tr_b16, 4 rows by 64 bytes for 32 lanes); the
-// two swizzles spread the rows of one such read over all 64 banks.
+// channels (ds_read_b128, lane l row l % 32), values transposed (ds_read_b64_tr_b16, 4 rows by 64 bytes for 32 lanes);
+// the two swizzles spread the rows of one such read over all 64 banks.
 template <int D>
 struct Tile {
     static constexpr int CHUNKS = D / 8;
@@ -152,10 +153,10 @@ __device__ __forceinline__ uint2 lds_read_transposed(uint32_t at) {
                                          (__attribute__((address_space(3))) i16x4*)static_cast<uintptr_t>(at)));
 }
 
-// Copies of 64-row tiles straight into LDS (buffer_load_dwordx4 ... lds: 64 lanes' 16 bytes in a row from the address in
-// M0), by a workgroup of THREADS. A lane's place in LDS is fixed, so it fetches the chunk the swizzle puts there. Rows past the
-// sequence's end are outside the buffer resource (the whole offset is the lane's: the scalar one is no part of the check).
-// The copies of a tile complete at the workgroup's next tile_barrier.
+// Copies of 64-row tiles straight into LDS (buffer_load_dwordx4 ... lds: 64 lanes' 16 bytes in a row from the address
+// in M0), by a workgroup of THREADS. A lane's place in LDS is fixed, so it fetches the chunk the swizzle puts there.
+// Rows past the sequence's end are outside the buffer resource (the whole offset is the lane's: the scalar one is no
+// part of the check). The copies of a tile complete at the workgroup's next tile_barrier.
 template <int D, int THREADS>
 struct TileCopy {
     static constexpr int CHUNKS = D / 8, N = 64 * CHUNKS / THREADS, ROWS = THREADS / CHUNKS;  // rows per instruction
