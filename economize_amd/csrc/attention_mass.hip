@@ -9,8 +9,8 @@
 // they read the same ones at the same time. Long walks are cut by heads, each a workgroup of its own, summed by
 // mass_sum_kernel.
 //
-// Bound by the matrix instructions and the exponentials together: 32768 tokens, 32 heads of 128 on 8, take 3.9 ms, 1.13
-// PFLOP/s (1.31 in a large library product); 4 prompts of 1000 to 8192 tokens 460 us, 1.01. The last 64 queries of 16
+// Bound by the matrix instructions and the exponentials together: 32768 tokens, 32 heads of 128 on 8, take 4.0 ms, 1.10
+// PFLOP/s (1.31 in a large library product); 4 prompts of 1000 to 8192 tokens 465 us, 1.00. The last 64 queries of 16
 // prompts of 501 to 8000 tokens (16 heads of 64 on 4) take 29 us, four times their keys' HBM time: four steps to a
 // walk, whose fetches and barriers a workgroup waits for.
 

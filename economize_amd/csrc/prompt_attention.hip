@@ -12,9 +12,9 @@
 // 64 each, one step ahead; the scores of a tile are computed under the exponentials of the one before.
 //
 // Long sequences are bound by the matrix instructions and the power they draw: 32768 tokens, 32 heads of 128 on 8, take
-// 8.0 ms, 1.1 PFLOP/s (a large library product reaches 1.31; on zeros, which draw less, a build of 8.5 ms took 6.4).
+// 8.1 ms, 1.08 PFLOP/s (a large library product reaches 1.31; on zeros, which draw less, a build of 8.5 ms took 6.4).
 // Short ones are bound by a row tile's chain of bounds, keys, products and outputs (6 us beside 1.3 us a tile of keys):
-// 24 prompts of 1 to 2047 tokens take 366 us, 0.77 PFLOP/s. Heads of 64 are bound by the exponentials (8 x 4000 tokens:
+// 24 prompts of 1 to 2047 tokens take 370 us, 0.76 PFLOP/s. Heads of 64 are bound by the exponentials (8 x 4000 tokens:
 // 0.80 PFLOP/s), heads of 256 by registers, which leave one wave to a SIMD (0.59). 64 rows to a wave read LDS half as
 // often but left no registers to overlap products and exponentials (32768 tokens 10 ms where 32 rows took 8.5).
 
@@ -324,8 +324,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : D == 128 ? 2 : 3) void prom
     }
 }
 
-// The parts of the rows whose keys were cut (6 prompt chunks of 100 to 612 tokens in two parts: 12 us of 131, at 2.5
-// TB/s): four channels to a lane, JOINED rows of a row tile to a workgroup.
+// The parts of the rows whose keys were cut (6 prompt chunks of 100 to 612 tokens in two parts: 8 us of 134): four
+// channels to a lane, JOINED rows of a row tile to a workgroup.
 constexpr int JOINED = 32;
 
 template <int D, int FMT>
