@@ -48,7 +48,7 @@ struct WorkOrder {
 // half of the CUs' time idle).
 inline WorkOrder work_order(int sequences, int kv_heads, int64_t tiles, int parts, int64_t bytes) {
     const int64_t pairs = static_cast<int64_t>(sequences) * kv_heads;
-    const int64_t most_tiles = (1 << 23) / (pairs * parts);
+    const int64_t most_tiles = (1 << 23) / (pairs * parts);  // (a launch holds fewer than 2^32 threads)
     tiles = tiles < most_tiles ? tiles : most_tiles;
     WorkOrder o;
     o.pairs = static_cast<int>(pairs);

@@ -474,8 +474,8 @@ int eco_kivi_packed_decode(const void* q, int32_t q_format, int64_t sq_b, int64_
 /* Causal attention of every sequence's queries over its own keys: out [q_rows, Hq, D] and lse [Hq, sl_h] (optional, fp32:
  * the logarithm of the softmax denominator, sinks [Hq] included). A query that sees no key gives 0 and lse -inf (its
  * sink's logit with sinks). Rows of no sequence: 0 and -inf with fill, else left as they are. The workspace (sized
- * for the same bounds; NULL where its size is 0) holds the parts of rows whose keys are cut. At most 65535 sequences times
- * KV heads. */
+ * for the same bounds; NULL where its size is 0) holds the parts of rows whose keys are cut, and need not be cleared. The
+ * outputs may overlap neither each other nor the keys and values. At most 65535 sequences times KV heads. */
 size_t eco_prompt_attention_workspace_size(int32_t sequences, int64_t q_rows, int32_t max_queries, int32_t max_keys,
                                            int32_t q_heads, int32_t kv_heads, int32_t head_dim);
 int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, const void* v,
@@ -488,8 +488,8 @@ int eco_prompt_attention(const void* q, int32_t format, int64_t sq_t, int64_t sq
 
 /* The attention weight every key received: mass[h, j] (fp32 [Hkv, sm_h]) = the sum over the queries that see key j (with
  * window > 0 the last `window` of its sequence) and the query heads of KV head h of exp(score - lse). Keys of no
- * sequence: 0 with fill, else left as they are. The workspace (sized for the same max_queries) holds the sums of long
- * walks' parts. At most 65535 sequences times KV heads. */
+ * sequence: 0 with fill, else left as they are. The workspace (sized for the same max_queries and window) holds the sums of
+ * long walks' parts, and need not be cleared. At most 65535 sequences times KV heads. */
 size_t eco_attention_mass_workspace_size(int32_t max_queries, int64_t k_rows, int32_t window, int32_t q_heads,
                                          int32_t kv_heads);
 int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h, const void* k, int64_t sk_t,
@@ -505,7 +505,8 @@ int eco_attention_mass(const void* q, int32_t format, int64_t sq_t, int64_t sq_h
  *
  * Fills it from packed prompts, row b from key rows [begin[b], end[b]): of its n tokens every KV head keeps all if they
  * fit, else the first, the newest and those of greatest mass [Hkv, sm_h] among the rest (equal: the lower index; a NaN is
- * the least), in token order. Slots past the count are left as they are. max_tokens sizes the launch. */
+ * the least), in token order. Slots past the count are left as they are. max_tokens sizes the launch. The prompt
+ * lies in memory apart from the cache's. At most 65535 rows times KV heads, 2^25 slots and 2^30 - 1 in all. */
 int eco_evict_prompt(const void* k, const void* v, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h,
                      const float* mass, int64_t sm_h, const int32_t* begin, const int32_t* end, int64_t rows,
                      int32_t max_tokens, void* keys, void* values, float* score, int32_t* position, int32_t* count,
