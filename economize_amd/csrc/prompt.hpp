@@ -78,7 +78,7 @@ struct PromptParams {
     int q_heads, kv_heads, groups, head_dim;
     Divisor per_group, per_kv, per_part;  // over the groups, the KV heads, the row tiles of a part
     WorkOrder order;  // (sequences of more row tiles than the launch holds loop over them)
-    int parts;                     // a row tile's keys are cut into up to so many
+    int parts, part_shift;         // a row tile's keys are cut into up to so many, of 1 << part_shift tiles or more
     float *part_out, *part_stats;  // [parts, q_rows, Hq, D] and [.., 2], of the row tiles that were cut
     float scale, softcap;
 };

@@ -29,11 +29,9 @@ constexpr int ROWS = WAVES * 32;  // rows of a tile
 
 constexpr float NEVER = -1e30f;  // running maximum before the first key (log2 units)
 
-constexpr int MIN_PART = 8;  // tiles of 64 keys a part holds at least: its rows' sums are written and read once more
-
 // The parts of a row tile that sees so many tiles of keys, and the first tile of a part.
 __device__ __forceinline__ int parts_of(const PromptParams& p, int key_tiles) {
-    const int n = key_tiles / MIN_PART;
+    const int n = key_tiles >> p.part_shift;
     return n < 1 ? 1 : n < p.parts ? n : p.parts;
 }
 
@@ -401,18 +399,27 @@ constexpr int64_t MOST_PART_BYTES = 1 << 29;
 // the LDS), their keys are cut into up to so many parts. With twice the workgroups and with these, 32 heads of 128 on 8:
 // a prompt of 4000 tokens 178 and 146 us, 512 tokens behind 8000 98 and 89, 128 behind 16000 82 and 63; 16 heads of 256:
 // a prompt of 2000 tokens 111 and 98, 512 behind 30000 410 and 376.
-int most_parts(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads, int head_dim) {
-    if (q_rows == 0) return 1;
+//
+// A part holds at least eight tiles of 64 keys, since its rows' sums are written and read once more, or four where the
+// row tiles are an eighth of those workgroups or less (with eight and four: one token behind 1000 keys 27 and 17 us, 16
+// behind 1000 in 4 sequences 28 and 22, but a prompt of 1000 tokens 29 and 35).
+struct Cut {
+    int parts, shift;  // up to so many parts, of at least 1 << shift tiles
+};
+
+Cut cut_of(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads, int head_dim) {
+    if (q_rows == 0) return {1, 0};
     const int64_t groups = q_heads / kv_heads;
     const int64_t by_longest = (max_queries * groups + ROWS - 1) / ROWS * sequences;
     const int64_t by_rows = q_rows * groups / ROWS + sequences;
     const int64_t row_tiles = (by_longest < by_rows ? by_longest : by_rows) * kv_heads;
-    int64_t most = static_cast<int64_t>(max_keys) / (64 * MIN_PART);
+    const int64_t resident = head_dim == 256 ? 256 : 512;
+    const int shift = 8 * row_tiles <= resident ? 2 : 3;
+    int64_t most = static_cast<int64_t>(max_keys) / (64 << shift);
     const int64_t fit = MOST_PART_BYTES / static_cast<int64_t>(part_bytes(1, q_rows, q_heads, head_dim + 2));
     most = most < fit ? most : fit;
-    const int64_t resident = head_dim == 256 ? 256 : 512;
     const int64_t parts = row_tiles > 0 ? (resident + row_tiles - 1) / row_tiles : 1;
-    return static_cast<int>(parts < 1 || most < 1 ? 1 : parts < most ? parts : most);
+    return {static_cast<int>(parts < 1 || most < 1 ? 1 : parts < most ? parts : most), shift};
 }
 
 template <int D, int FMT>
@@ -449,13 +456,15 @@ int launch_dim(const PromptParams& p, int max_queries, int max_keys, hipStream_t
 
 size_t prompt_attention_workspace(int sequences, int64_t q_rows, int max_queries, int max_keys, int q_heads, int kv_heads,
                                   int head_dim) {
-    const int parts = most_parts(sequences, q_rows, max_queries, max_keys, q_heads, kv_heads, head_dim);
+    const int parts = cut_of(sequences, q_rows, max_queries, max_keys, q_heads, kv_heads, head_dim).parts;
     return parts == 1 ? 0 : part_bytes(parts, q_rows, q_heads, head_dim + 2);
 }
 
 int prompt_attention(PromptParams p, int format, int max_queries, int max_keys, void* workspace, size_t workspace_bytes,
                      hipStream_t stream) {
-    p.parts = most_parts(p.rows.sequences, p.rows.q_rows, max_queries, max_keys, p.q_heads, p.kv_heads, p.head_dim);
+    const Cut cut = cut_of(p.rows.sequences, p.rows.q_rows, max_queries, max_keys, p.q_heads, p.kv_heads, p.head_dim);
+    p.parts = cut.parts;
+    p.part_shift = cut.shift;
     if (p.parts > 1 && (!workspace || workspace_bytes < part_bytes(p.parts, p.rows.q_rows, p.q_heads, p.head_dim + 2)))
         return fail("prompt attention: the workspace is too small");
     p.part_out = static_cast<float*>(workspace);
